@@ -10,12 +10,14 @@ extension is missing this raises. On CPU tensors the op evaluates the fp32 oracl
 from __future__ import annotations
 
 import math
+from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
 
 from . import reference as R
 from .layout import split_gate_up
+from .quant import dequantize_w4, quantize_w4  # noqa: F401  (public names of the 4-bit weights)
 
 
 def _cuda():
@@ -206,3 +208,105 @@ def ngram_embed(ids: torch.Tensor, table: torch.Tensor, orders, n_hash: int) -> 
     if ids.is_cuda:
         return _cuda().ngram_embed(ids, table, orders, n_hash)
     return R.ngram_embed(ids, table, orders, n_hash)
+
+
+# ------------------------------------------------------------------------ quantised serving path
+#
+# A paged KV cache in 8 bits, its block tables, and products with 4-bit weights. None of them has a
+# backward pass; the ones that take activations refuse inputs that require a gradient.
+
+
+def _serving_only(name: str, *tensors) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} has no backward pass")
+
+
+class BlockPlan(NamedTuple):
+    """One step of a paged cache (all int32). Rows behind the last new token have slot and request
+    -1 and position 0. ``status`` is 0, or has the bits 1 (too few free pages), 2 (a request outgrows
+    its row of the table), 4 (more new tokens than rows), 8 (a negative length or a bad free count):
+    then nothing was placed, the tables are unchanged and ``lens`` / ``free_count`` are the old ones."""
+
+    lens: torch.Tensor        # [R] lengths with the new tokens
+    free_count: torch.Tensor  # [1] free pages left
+    starts: torch.Tensor      # [R + 1] first row of each request's new tokens
+    slots: torch.Tensor       # [rows] page * page_size + offset of each new token
+    requests: torch.Tensor    # [rows] its request
+    positions: torch.Tensor   # [rows] its position in the request
+    status: torch.Tensor      # [1]
+
+
+def block_tables_extend(tables, lens, new_lens, free_pages, free_count, page_size: int, rows: int) -> BlockPlan:
+    """Give ``new_lens [R]`` further tokens of each request their pages and rows, on the device.
+
+    ``tables [R, width]`` (request r's pages, in order; written in place), ``lens [R]`` (tokens that
+    are cached), ``free_pages`` (a stack of unused pages: the first ``free_count [1]`` entries, taken
+    from the end), all int32. ``rows`` is the number of rows of the step (the new tokens of all
+    requests, packed, and padding). Only ``tables`` changes, so calling it again gives the same plan;
+    the caller keeps the plan's ``lens`` and ``free_count`` when it takes the step. Up to 4096
+    requests."""
+    if tables.is_cuda:
+        return BlockPlan(*_cuda().ext().block_tables_extend(tables, lens, new_lens, free_pages, free_count, page_size,
+                                                            rows))
+    return BlockPlan(*R.block_tables_extend(tables, lens, new_lens, free_pages, free_count, page_size, rows))
+
+
+def block_tables_release(tables, lens, done, free_pages, free_count, page_size: int) -> torch.Tensor:
+    """Push the pages of the requests marked in ``done [R]`` (bool) onto the free stack and empty
+    them (``lens`` 0, table entries -1), in place. Returns a status ``[1]`` like ``BlockPlan``'s; if
+    it is not 0 nothing changed."""
+    if tables.is_cuda:
+        return _cuda().ext().block_tables_release(tables, lens, done, free_pages, free_count, page_size)
+    return R.block_tables_release(tables, lens, done, free_pages, free_count, page_size)
+
+
+def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, slots) -> None:
+    """Write rows of keys and values (``[rows, kv_heads, head_dim]`` bf16, head_dim 64 or 128) to
+    their slots of a cache of e4m3 codes ``[pages, kv_heads, page, head_dim]`` (page 32, 64 or 128)
+    with fp32 scales ``[pages, kv_heads]``, in place.
+
+    Scales are powers of two. A row at offset 0 starts its page anew; rows further on keep the page's
+    scale or raise it, and raising it rescales the codes before them. Values that are not finite are
+    stored as NaN. Rows with a slot outside the cache (the padding's -1) are skipped. The rows of one
+    page must be consecutive rows with ascending slots, as a ``BlockPlan`` gives them, and a page must
+    belong to one request: two runs of rows in one page would race for its scale."""
+    _serving_only("kv8_append", k, v)
+    if k.is_cuda:
+        _cuda().ext().kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, slots)
+    else:
+        R.kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, slots)
+
+
+def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, tables, lens, *, starts=None, scale: float | None = None,
+                  out=None) -> torch.Tensor:
+    """Causal attention of the requests' newest rows over their cached tokens (GQA), ``[rows, heads,
+    head_dim]`` bf16.
+
+    ``lens [R]`` counts the cached tokens with the new ones, which are already appended. Rows
+    ``starts[r] .. starts[r + 1]`` of ``q`` are the last tokens of request r; without ``starts`` each
+    request has one row. A row that sees no token is zero. A row that sees a page outside the cache,
+    or a request longer than its table, is NaN. Rows behind the last request are left as they were in
+    ``out``, and are zero without it. ``starts`` must ascend within ``0 .. rows``."""
+    _serving_only("kv8_attention", q)
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    if q.is_cuda:
+        return _cuda().ext().kv8_attention(q, k_cache, v_cache, k_scale, v_scale, tables, lens, starts, scale, out)
+    return R.kv8_attention(q, k_cache, v_cache, k_scale, v_scale, tables, lens, starts, scale, out)
+
+
+def linear_w4(x, codes, scales, *, residual=None, glu: bool = False) -> torch.Tensor:
+    """``x [T, K] @ w^T`` with the 4-bit weights of ``quantize_w4`` (+ ``residual [T, N]``), bf16.
+
+    ``glu``: the weight holds block-interleaved gate and up rows (``ops.layout``) and the result is
+    ``silu(gate) * up`` ``[T, N / 2]``. Up to 64 rows the weights stay in 4 bits on their way to the
+    tensor cores; more rows run the dense GEMM on weights written out in bf16 (each rounded once
+    more, and a temporary of ``2 N K`` bytes)."""
+    _serving_only("linear_w4", x, residual)
+    if not x.is_cuda:
+        return R.linear_w4(x, codes, scales, residual, glu)
+    if x.shape[0] <= 64:
+        return _cuda().ext().linear_w4(x, codes, scales, residual, glu)
+    return _cuda().linear_w4_dense(x, codes, scales, residual, glu)

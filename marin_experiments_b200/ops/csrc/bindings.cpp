@@ -16,7 +16,7 @@ namespace {
 
 cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
-void check_code(int code, const char* what) { TORCH_CHECK(code == 0, what, ": launch failed (code ", code, ")"); }
+void check_code(int code, const char* what) { TORCH_CHECK(code == 0, what, ": launch failed (code ", std::to_string(code), ")"); }
 
 void check_2d_bf16(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");

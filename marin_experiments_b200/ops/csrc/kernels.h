@@ -170,6 +170,53 @@ int launch_decode_attention(const void* q, const void* ck, const void* cv, const
                             int hd, int Lmax, float scale, int nsplit, float* part_ml, float* part_acc, void* out,
                             cudaStream_t st);
 
+// -------------------------------------------------- block tables of a paged cache (block_tables.cu)
+constexpr int kTablesMaxRequests = 4096;
+// status bits of a refused step (nothing is changed)
+constexpr int kTablesNoPages = 1;      // fewer free pages than the step needs
+constexpr int kTablesTooLong = 2;      // a request outgrows its row of the table
+constexpr int kTablesTooManyRows = 4;  // more new tokens than rows
+constexpr int kTablesBadInput = 8;     // a negative length, or a free count outside the stack
+int launch_block_tables_extend(int* tables, int width, const int* lens, const int* grow, int R, const int* free_pages,
+                               int capacity, const int* free_count, int page, int rows, int* lens_out, int* count_out,
+                               int* starts, int* slots, int* requests, int* positions, int* status, cudaStream_t st);
+int launch_block_tables_release(int* tables, int width, int* lens, const uint8_t* done, int R, int* free_pages,
+                                int capacity, int* free_count, int page, int* status, cudaStream_t st);
+
+// ------------------------------------------------------------------ paged 8-bit KV cache (kv8.cu)
+// Cache [pages, hkv, page, hd] e4m3, scales [pages, hkv] (powers of two).
+struct Kv8Cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int pages, hkv, page, hd;
+};
+int launch_kv8_append(const Kv8Cache& c, const void* k, const void* v, long k_tok, long v_tok, const int* slots,
+                      int rows, cudaStream_t st);
+struct Kv8Attention {
+  const void* q;  // [rows, H, hd] bf16, heads contiguous
+  long q_tok;
+  const int* tables;  // [R, width]
+  const int* lens;    // [R], the new tokens included
+  const int* starts;  // [R + 1] first row of each request, or null: row r is request r's one token
+  void* out;          // [rows, H, hd] bf16 contiguous
+  int rows, H, R, width, zero_tail;
+  float scale;
+  float* work;  // kv8_attention_work floats
+  int grid;     // kv8_attention_grid
+};
+// CTAs of the attention for a call of these sizes (an upper bound on its work), or -1 if the sizes
+// are outside what it indexes; floats of its workspace.
+int kv8_attention_grid(int rows, int H, int hkv, int R, int width, int page, int sms);
+long kv8_attention_work(int grid, int R, int hd);
+int launch_kv8_attention(const Kv8Cache& c, const Kv8Attention& a, cudaStream_t st);
+
+// ----------------------------------------------------------------------- 4-bit weights (w4.cu)
+int launch_linear_w4(const void* x, long x_tok, const void* codes, const void* scales, const void* residual, long r_tok,
+                     void* out, int T, int N, int K, int group, int glu, cudaStream_t st);
+int launch_dequant_w4(const void* codes, const void* scales, void* out, int N, int K, int group, cudaStream_t st);
+
 // ------------------------------------------------------------------- hashed n-gram embedding (ngram.cu)
 int launch_ngram_fwd(const int64_t* ids, int B, int S, const int* orders, int n_orders, int n_hash, long buckets,
                      const void* table, int rank, void* out, cudaStream_t st);

@@ -1,5 +1,6 @@
 // Torch bindings of the row-wise, attention, MoE and optimizer kernels.
 #include <algorithm>
+#include <string>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -29,7 +30,9 @@ template <class T>
 T* ptr(const OptT& t) {
   return t.has_value() ? reinterpret_cast<T*>(t->data_ptr()) : nullptr;
 }
-void ok(int code, const char* what) { TORCH_CHECK(code == 0, what, " failed (", code, ")"); }
+// Messages get text only: a number put through a C++ stream here can end the process (the stream's
+// locale facets are not this library's own) instead of raising.
+void ok(int code, const char* what) { TORCH_CHECK(code == 0, what, " failed (", std::to_string(code), ")"); }
 
 // ------------------------------------------------------------------------------------ rows
 void rmsnorm_fwd(const Tensor& x, const Tensor& w, const Tensor& y, const Tensor& rstd, double eps) {
@@ -543,6 +546,216 @@ void decode_attention(const Tensor& q, const Tensor& ck, const Tensor& cv, const
      "decode_attention");
 }
 
+// ------------------------------------------------- block tables, 8-bit cache and 4-bit weights
+void cuda_i32(const Tensor& t, const char* n) {
+  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kInt && t.is_contiguous(), n,
+              " must be a contiguous CUDA int32 tensor");
+}
+void same_device(const Tensor& a, std::initializer_list<const Tensor*> rest) {
+  for (auto* t : rest) TORCH_CHECK(t->device() == a.device(), "all tensors must be on one device");
+}
+bool overlaps(const Tensor& a, const Tensor& b) {
+  const char *x = (const char*)a.data_ptr(), *y = (const char*)b.data_ptr();
+  return x < y + b.nbytes() && y < x + a.nbytes();
+}
+
+std::vector<Tensor> block_tables_extend(const Tensor& tables, const Tensor& lens, const Tensor& grow,
+                                        const Tensor& free_pages, const Tensor& free_count, int64_t page,
+                                        int64_t rows) {
+  cuda_i32(tables, "tables"); cuda_i32(lens, "lens"); cuda_i32(grow, "new_lens");
+  cuda_i32(free_pages, "free_pages"); cuda_i32(free_count, "free_count");
+  same_device(tables, {&lens, &grow, &free_pages, &free_count});
+  need(tables.dim() == 2 && lens.dim() == 1 && grow.dim() == 1 && free_pages.dim() == 1 && free_count.numel() == 1,
+       "tables [R, width], lens [R], new_lens [R], free_pages [pages], free_count [1]");
+  const int64_t R = tables.size(0);
+  need(lens.size(0) == R && grow.size(0) == R, "one length and one new length for each row of the tables");
+  need(R >= 1 && R <= mxk::kTablesMaxRequests, "between 1 and 4096 requests");
+  need(page >= 1 && rows >= 0 && rows < (1LL << 31) - 1, "page must be positive and rows not negative");
+  need(free_pages.numel() * page < (1LL << 31) && tables.size(1) * page < (1LL << 31),
+       "a pool or a table of 2^31 tokens or more");
+  c10::cuda::CUDAGuard g(tables.device());
+  // one buffer: lens [R], starts [R + 1], free_count, status, slots, requests, positions [rows]
+  Tensor buf = at::empty({2 * R + 3 + 3 * rows}, tables.options());
+  int* b = buf.data_ptr<int>();
+  int* sl = b + 2 * R + 3;
+  ok(mxk::launch_block_tables_extend(tables.data_ptr<int>(), (int)tables.size(1), lens.data_ptr<int>(),
+                                     grow.data_ptr<int>(), (int)R, free_pages.data_ptr<int>(),
+                                     (int)free_pages.numel(), free_count.data_ptr<int>(), (int)page, (int)rows, b,
+                                     b + 2 * R + 1, b + R, sl, sl + rows, sl + 2 * rows, b + 2 * R + 2, stream()),
+     "block_tables_extend");
+  auto part = [&](int64_t at, int64_t n) { return buf.narrow(0, at, n); };
+  const int64_t s = 2 * R + 3;
+  return {part(0, R), part(2 * R + 1, 1), part(R, R + 1), part(s, rows), part(s + rows, rows),
+          part(s + 2 * rows, rows), part(2 * R + 2, 1)};
+}
+
+Tensor block_tables_release(const Tensor& tables, const Tensor& lens, const Tensor& done, const Tensor& free_pages,
+                            const Tensor& free_count, int64_t page) {
+  cuda_i32(tables, "tables"); cuda_i32(lens, "lens"); cuda_i32(free_pages, "free_pages");
+  cuda_i32(free_count, "free_count");
+  need(done.is_cuda() && done.scalar_type() == at::kBool && done.is_contiguous(), "done must be a CUDA bool tensor");
+  same_device(tables, {&lens, &done, &free_pages, &free_count});
+  need(tables.dim() == 2 && lens.dim() == 1 && done.dim() == 1 && free_pages.dim() == 1 && free_count.numel() == 1,
+       "tables [R, width], lens [R], done [R], free_pages [pages], free_count [1]");
+  const int64_t R = tables.size(0);
+  need(lens.size(0) == R && done.size(0) == R, "one length and one mark for each row of the tables");
+  need(R >= 1 && R <= mxk::kTablesMaxRequests, "between 1 and 4096 requests");
+  need(page >= 1, "page must be positive");
+  c10::cuda::CUDAGuard g(tables.device());
+  Tensor status = at::empty({1}, tables.options());
+  ok(mxk::launch_block_tables_release(tables.data_ptr<int>(), (int)tables.size(1), lens.data_ptr<int>(),
+                                      (const uint8_t*)done.data_ptr(), (int)R, free_pages.data_ptr<int>(),
+                                      (int)free_pages.numel(), free_count.data_ptr<int>(), (int)page,
+                                      status.data_ptr<int>(), stream()),
+     "block_tables_release");
+  return status;
+}
+
+mxk::Kv8Cache kv8_cache(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs) {
+  for (auto* t : {&k, &v}) {
+    need(t->is_cuda() && t->scalar_type() == at::kFloat8_e4m3fn && t->dim() == 4 && t->is_contiguous(),
+         "caches must be contiguous CUDA float8_e4m3fn tensors [pages, kv_heads, page, head_dim]");
+    aligned16(*t, "cache");
+  }
+  for (auto* t : {&ks, &vs}) {
+    cuda_f32(*t, "cache scales");
+    contig(*t, "cache scales");
+    need(t->dim() == 2 && t->size(0) == k.size(0) && t->size(1) == k.size(1), "cache scales are [pages, kv_heads]");
+  }
+  need(k.sizes() == v.sizes(), "key and value caches must have one shape");
+  same_device(k, {&v, &ks, &vs});
+  need(k.size(3) == 64 || k.size(3) == 128, "head_dim must be 64 or 128");
+  need(k.size(2) == 32 || k.size(2) == 64 || k.size(2) == 128, "page must be 32, 64 or 128 tokens");
+  need(k.size(0) >= 1 && k.size(1) >= 1 && k.size(1) <= 65535 && k.size(0) * k.size(2) < (1LL << 31),
+       "a cache of 1 to 2^31 tokens with 1 to 65535 heads");
+  return {k.data_ptr(), v.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(),
+          (int)k.size(0), (int)k.size(1), (int)k.size(2), (int)k.size(3)};
+}
+
+// Rows [n, heads, hd] bf16 whose heads are contiguous; the row stride is free.
+long rows_of(const Tensor& t, int64_t heads, int64_t hd, const char* n) {
+  cuda_bf16(t, n);
+  TORCH_CHECK(t.dim() == 3 && t.size(1) == heads && t.size(2) == hd, n, " must be [rows, heads, head_dim]");
+  if (t.numel() == 0) return heads * hd;
+  TORCH_CHECK(t.stride(2) == 1 && (heads == 1 || t.stride(1) == hd), n, ": heads must be contiguous");
+  const int64_t s = t.size(0) == 1 ? heads * hd : t.stride(0);
+  TORCH_CHECK(s % 8 == 0 && s >= 0, n, ": the row stride must be a multiple of 8");
+  aligned16(t, n);
+  return s;
+}
+
+void kv8_append(const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor& vc, const Tensor& ks,
+                const Tensor& vs, const Tensor& slots) {
+  const mxk::Kv8Cache c = kv8_cache(kc, vc, ks, vs);
+  const long kt = rows_of(k, c.hkv, c.hd, "k"), vt = rows_of(v, c.hkv, c.hd, "v");
+  cuda_i32(slots, "slots");
+  same_device(kc, {&k, &v, &slots});
+  need(k.size(0) == v.size(0) && slots.dim() == 1 && slots.size(0) == k.size(0), "one slot for each row of k and v");
+  need(k.size(0) < (1LL << 31) - 64, "too many rows");
+  c10::cuda::CUDAGuard g(kc.device());
+  ok(mxk::launch_kv8_append(c, k.data_ptr(), v.data_ptr(), kt, vt, slots.data_ptr<int>(), (int)k.size(0), stream()),
+     "kv8_append");
+}
+
+Tensor kv8_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs,
+                     const Tensor& tables, const Tensor& lens, const OptT& starts, double scale, const OptT& out) {
+  const mxk::Kv8Cache c = kv8_cache(kc, vc, ks, vs);
+  need(q.dim() == 3 && q.size(1) >= 1 && q.size(1) % c.hkv == 0, "q must be [rows, heads, head_dim], heads a multiple of kv_heads");
+  const int64_t T = q.size(0), H = q.size(1);
+  const long qt = rows_of(q, H, c.hd, "q");
+  cuda_i32(tables, "tables"); cuda_i32(lens, "lens");
+  same_device(kc, {&q, &tables, &lens});
+  need(tables.dim() == 2 && lens.dim() == 1 && lens.size(0) == tables.size(0) && tables.size(1) >= 1,
+       "tables must be [R, width] and lens [R]");
+  const int64_t R = tables.size(0);
+  if (starts.has_value()) {
+    cuda_i32(*starts, "starts");
+    same_device(kc, {&*starts});
+    need(starts->dim() == 1 && starts->size(0) == R + 1, "starts must be [R + 1]");
+  } else {
+    need(T == R, "without starts there is one row for each request");
+  }
+  need(T < (1LL << 31) - 64 && R >= 1 && R <= mxk::kTablesMaxRequests && H <= 65535, "between 1 and 4096 requests");
+  c10::cuda::CUDAGuard g(kc.device());
+  Tensor o;
+  if (out.has_value()) {
+    o = *out;
+    cuda_bf16(o, "out");
+    contig(o, "out");
+    aligned16(o, "out");
+    same_device(kc, {&o});
+    need(o.sizes() == q.sizes(), "out must have q's shape");
+    need(!overlaps(o, kc) && !overlaps(o, vc) && (T == 0 || !overlaps(o, q)), "out must not overlap an input");
+  } else {
+    o = at::empty(q.sizes(), q.options());
+  }
+  if (T == 0) return o;
+  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const int grid = mxk::kv8_attention_grid((int)T, (int)H, c.hkv, (int)R, (int)tables.size(1), c.page, sms);
+  need(grid > 0, "rows, heads and table width are beyond what one call indexes");
+  Tensor work = at::empty({mxk::kv8_attention_work(grid, (int)R, c.hd)}, ks.options());
+  mxk::Kv8Attention a{q.data_ptr(), qt, tables.data_ptr<int>(), lens.data_ptr<int>(),
+                      starts.has_value() ? starts->data_ptr<int>() : nullptr, o.data_ptr(), (int)T, (int)H, (int)R,
+                      (int)tables.size(1), starts.has_value() && !out.has_value(), (float)scale,
+                      work.data_ptr<float>(), grid};
+  ok(mxk::launch_kv8_attention(c, a, stream()), "kv8_attention");
+  return o;
+}
+
+// The group of 4-bit weights, after their checks.
+int w4_group(const Tensor& codes, const Tensor& scales) {
+  need(codes.is_cuda() && codes.scalar_type() == at::kInt && codes.dim() == 2 && codes.is_contiguous(),
+       "codes must be a contiguous CUDA int32 tensor [N, K / 8]");
+  cuda_bf16(scales, "scales"); contig(scales, "scales");
+  same_device(codes, {&scales});
+  aligned16(codes, "codes");
+  const int64_t N = codes.size(0), K = codes.size(1) * 8;
+  need(N >= 1 && K >= 128 && K % 128 == 0 && N < (1LL << 31) - 64 && K < (1LL << 30), "K must be a multiple of 128");
+  need(scales.dim() == 2 && scales.size(0) == N && scales.size(1) >= 1 && K % scales.size(1) == 0,
+       "scales must be [N, K / group]");
+  const int64_t group = K / scales.size(1);
+  need(group == 32 || group == 64 || group == 128, "group must be 32, 64 or 128");
+  return (int)group;
+}
+
+Tensor linear_w4(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptT& residual, bool glu) {
+  const int group = w4_group(codes, scales);
+  const int64_t N = codes.size(0), K = codes.size(1) * 8;
+  auto rows = [&](const Tensor& t, int64_t cols, int64_t align, const char* n) {
+    cuda_bf16(t, n);
+    same_device(codes, {&t});
+    TORCH_CHECK(t.dim() == 2 && t.size(1) == cols && (t.size(1) == 1 || t.stride(1) == 1), n, " must be rows of ", std::to_string(cols));
+    const int64_t s = t.size(0) <= 1 ? cols : t.stride(0);
+    TORCH_CHECK(s >= 0 && s % align == 0, n, ": the row stride must be a multiple of ", std::to_string(align));
+    return (long)s;
+  };
+  const long xt = rows(x, K, 8, "x");
+  aligned16(x, "x");
+  need(x.size(0) <= 64, "linear_w4 takes up to 64 rows");
+  need(!glu || (N % 256 == 0 && !residual.has_value()), "glu: rows in blocks of 128 gate and 128 up, and no residual");
+  long rt = 0;
+  if (residual.has_value()) {
+    rt = rows(*residual, N, 1, "residual");
+    need(residual->size(0) == x.size(0), "one residual row for each row of x");
+  }
+  c10::cuda::CUDAGuard g(codes.device());
+  Tensor out = at::empty({x.size(0), glu ? N / 2 : N}, x.options());
+  ok(mxk::launch_linear_w4(x.data_ptr(), xt, codes.data_ptr(), scales.data_ptr(), ptr<const void>(residual), rt,
+                           out.data_ptr(), (int)x.size(0), (int)N, (int)K, group, glu, stream()),
+     "linear_w4");
+  return out;
+}
+
+Tensor dequant_w4(const Tensor& codes, const Tensor& scales) {
+  const int group = w4_group(codes, scales);
+  c10::cuda::CUDAGuard g(codes.device());
+  Tensor out = at::empty({codes.size(0), codes.size(1) * 8}, scales.options());
+  ok(mxk::launch_dequant_w4(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), (int)codes.size(0),
+                            (int)codes.size(1) * 8, group, stream()),
+     "dequant_w4");
+  return out;
+}
+
 // -------------------------------------------------------------------- hashed n-gram embedding
 void ngram_fwd(const Tensor& ids, const Tensor& orders, int64_t n_hash, int64_t buckets, const Tensor& table,
                const Tensor& out) {
@@ -606,6 +819,12 @@ void register_ops(pybind11::module& m) {
   m.def("ngram_bwd", &ngram_bwd);
   m.def("kv_append", &kv_append);
   m.def("decode_attention", &decode_attention);
+  m.def("block_tables_extend", &block_tables_extend);
+  m.def("block_tables_release", &block_tables_release);
+  m.def("kv8_append", &kv8_append);
+  m.def("kv8_attention", &kv8_attention);
+  m.def("linear_w4", &linear_w4);
+  m.def("dequant_w4", &dequant_w4);
   m.def("ipc_alloc", &ipc_alloc);
   m.def("ipc_open", &ipc_open);
   m.def("ipc_close", [](int64_t p) { return mxk::ipc_close(reinterpret_cast<void*>(p)); });

@@ -612,3 +612,33 @@ class _NgramEmbed(torch.autograd.Function):
 
 def ngram_embed(ids, table, orders, n_hash):
     return _NgramEmbed.apply(ids, table, tuple(orders), int(n_hash))
+
+
+# ------------------------------------------------------------------- 4-bit weights, many rows
+@torch.no_grad()
+def linear_w4_dense(x, codes, scales, residual, glu):
+    """``linear_w4`` for more rows than its kernel takes: bf16 weights and the dense GEMM."""
+    t, k = x.shape
+    n = codes.shape[0]
+    if x.dtype != BF16 or k != codes.shape[1] * 8:
+        raise ValueError(f"x must be bf16 [T, {codes.shape[1] * 8}], got {x.dtype} {tuple(x.shape)}")
+    if residual is not None and (glu or residual.dtype != BF16 or residual.shape != (t, n)):
+        raise ValueError(f"residual must be bf16 [{t}, {n}], without glu")
+    if glu and n % 256:
+        raise ValueError("glu: rows in blocks of 128 gate and 128 up")
+    x = _c(x)
+    w = ext().dequant_w4(codes, scales)
+    if glu:
+        h = torch.empty(t, n, dtype=BF16, device=x.device)
+        a = torch.empty(t, n // 2, dtype=BF16, device=x.device)
+        G.gemm(x, w, h, M=t, N=n, K=k, epi="swiglu", c2=a)
+        return a
+    pad = -n % 32  # the GEMM stores 32 columns at a time
+    if pad:
+        w = torch.cat([w, w.new_zeros(pad, k)])
+        out = G.linear(x, w)[:, :n]
+        return (out if residual is None else out + residual).contiguous()
+    if residual is None:
+        return G.linear(x, w)
+    out = torch.empty(t, n, dtype=BF16, device=x.device)
+    return G.linear(x, w, out=out, epi="resid", r=_c(residual))

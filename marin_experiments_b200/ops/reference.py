@@ -317,3 +317,132 @@ def ngram_embed(ids: torch.Tensor, table: torch.Tensor, orders, n_hash: int) -> 
             rows = table[oi].index_select(0, ngram_buckets(ids, n, h, buckets).reshape(-1))
             acc = rows if acc is None else acc + rows
     return acc / (len(orders) * n_hash)
+
+
+# --------------------------------------------------------------- paged 8-bit cache, 4-bit weights
+TABLES_NO_PAGES, TABLES_TOO_LONG, TABLES_TOO_MANY_ROWS, TABLES_BAD_INPUT = 1, 2, 4, 8
+
+
+def block_tables_extend(tables, lens, new_lens, free_pages, free_count, page: int, rows: int):
+    """See ``api.block_tables_extend``; returns its plan's fields in order."""
+    if tables.shape[0] < 1 or page < 1 or rows < 0:
+        raise ValueError("at least one request, a positive page and rows >= 0")
+    old, new, free = lens.tolist(), new_lens.tolist(), free_pages.tolist()
+    count, width = int(free_count), tables.shape[1]
+    status = 0 if 0 <= count <= len(free) else TABLES_BAD_INPUT
+    pairs = [(a, b) for a, b in zip(old, new) if a >= 0 and b >= 0]
+    if len(pairs) < len(old):
+        status |= TABLES_BAD_INPUT
+    if any(-(-(a + b) // page) > width for a, b in pairs):
+        status |= TABLES_TOO_LONG
+    if sum(b for _, b in pairs) > rows:
+        status |= TABLES_TOO_MANY_ROWS
+    if sum(-(-(a + b) // page) - -(-a // page) for a, b in pairs) > count:
+        status |= TABLES_NO_PAGES
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=tables.device)  # noqa: E731
+    starts, slots, requests, positions = [0], [], [], []
+    if not status:
+        for r, (a, b) in enumerate(zip(old, new)):
+            for c in range(-(-a // page), -(-(a + b) // page)):
+                count -= 1
+                tables[r, c] = free[count]
+            row = tables[r].tolist()
+            slots += [row[p // page] * page + p % page if row[p // page] >= 0 else -1 for p in range(a, a + b)]
+            requests += [r] * b
+            positions += range(a, a + b)
+            starts.append(starts[-1] + b)
+    else:
+        starts, new = [0] * (len(old) + 1), [0] * len(old)
+    pad = rows - len(slots)
+    return (ints([a + b for a, b in zip(old, new)]), ints([count]), ints(starts), ints(slots + [-1] * pad),
+            ints(requests + [-1] * pad), ints(positions + [0] * pad), ints([status]))
+
+
+def block_tables_release(tables, lens, done, free_pages, free_count, page: int):
+    """See ``api.block_tables_release``."""
+    n = [-(-a // page) if d else 0 for a, d in zip(lens.tolist(), done.tolist())]
+    count, status = int(free_count), 0
+    if not 0 <= count <= free_pages.numel() or min(n) < 0 or sum(n) > free_pages.numel() - count:
+        status |= TABLES_BAD_INPUT
+    if max(n) > tables.shape[1]:
+        status |= TABLES_TOO_LONG
+    if not status:
+        for r, c in enumerate(n):
+            free_pages[count:count + c] = tables[r, :c]
+            tables[r, :c] = -1
+            count += c
+        lens[done] = 0
+        free_count.fill_(count)
+    return torch.tensor([status], dtype=torch.int32, device=tables.device)
+
+
+def kv8_exponent(amax):
+    """Least e in [-110, 120] with ``amax <= 448 * 2^e`` (-110 for 0)."""
+    m, p = torch.frexp(amax.float())
+    e = torch.where(m <= 0.875, p - 9, p - 8).clamp(-110, 120)
+    return torch.where(amax > 0, e, torch.full_like(e, -110))
+
+
+def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, slots):
+    """See ``api.kv8_append``."""
+    page = k_cache.shape[2]
+    at, s = 0, slots.tolist()
+    while at < len(s):
+        pg, off = divmod(s[at], page)
+        if s[at] < 0 or pg >= k_cache.shape[0]:
+            at += 1
+            continue
+        n = 1
+        while at + n < len(s) and off + n < page and s[at + n] == s[at] + n:
+            n += 1
+        for x, cache, scale in ((k, k_cache, k_scale), (v, v_cache, v_scale)):
+            y = x[at:at + n].float().transpose(0, 1)  # [heads, n, dim]
+            fine = torch.isfinite(y)
+            need = torch.exp2(kv8_exponent(torch.where(fine, y.abs(), torch.zeros_like(y)).amax((1, 2))).float())
+            now = need if off == 0 else torch.maximum(need, scale[pg])
+            if off:
+                ratio = (scale[pg] / now)[:, None, None]
+                cache[pg, :, :off] = (cache[pg, :, :off].float() * ratio).to(cache.dtype)
+            y = torch.where(fine, y / now[:, None, None], torch.full_like(y, float("nan")))
+            cache[pg, :, off:off + n] = y.to(cache.dtype)
+            scale[pg] = now
+        at += n
+
+
+def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, tables, lens, starts=None, scale=None, out=None):
+    """See ``api.kv8_attention``."""
+    rows, h, hd = q.shape
+    pages, hkv, page, _ = k_cache.shape
+    scale = hd ** -0.5 if scale is None else scale
+    o = torch.zeros_like(q) if out is None else out
+    st = list(range(rows + 1)) if starts is None else starts.tolist()
+    for r, n in enumerate(lens.tolist()):
+        a, b = st[r], st[r + 1]
+        for i in range(a, b):
+            m = max(0, n - (b - 1 - i))
+            pg = tables[r, : -(-m // page)].long()
+            if m > tables.shape[1] * page or bool(((pg < 0) | (pg >= pages)).any()):
+                o[i] = float("nan")
+                continue
+            if m == 0:
+                o[i] = 0
+                continue
+            kk, vv = ((c[pg].float() * s[pg][..., None, None]).transpose(1, 2).reshape(-1, hkv, hd)[:m]
+                      for c, s in ((k_cache, k_scale), (v_cache, v_scale)))
+            sc = torch.einsum("grd,kgd->grk", q[i].float().view(hkv, h // hkv, hd), kk) * scale
+            o[i] = torch.einsum("grk,kgd->grd", torch.softmax(sc, -1), vv).reshape(h, hd).to(q.dtype)
+    return o
+
+
+def linear_w4(x, codes, scales, residual=None, glu: bool = False):
+    """See ``api.linear_w4``."""
+    from .layout import split_gate_up
+    from .quant import dequantize_w4
+
+    y = x.float() @ dequantize_w4(codes, scales).t()
+    if glu:
+        g, u = split_gate_up(y, y.shape[1] // 2)
+        y = activation(g, "silu") * u
+    if residual is not None:
+        y = y + residual.float()
+    return y.to(x.dtype)
