@@ -184,7 +184,8 @@ int launch_block_tables_release(int* tables, int width, int* lens, const uint8_t
                                 int capacity, int* free_count, int page, int* status, cudaStream_t st);
 
 // ------------------------------------------------------------------ paged 8-bit KV cache (kv8.cu)
-// Cache [pages, hkv, page, hd] e4m3, scales [pages, hkv] (powers of two).
+// Cache [pages, hkv, page, hd] e4m3, scales [pages, hkv] (powers of two). A negative v_scale marks a
+// page that holds NaN values.
 struct Kv8Cache {
   void* k;
   void* v;
@@ -205,11 +206,13 @@ struct Kv8Attention {
   float scale;
   float* work;  // kv8_attention_work floats
   int grid;     // kv8_attention_grid
+  int tile;     // kv8_attention_tile
 };
 // CTAs of the attention for a call of these sizes (an upper bound on its work), or -1 if the sizes
 // are outside what it indexes; floats of its workspace.
-int kv8_attention_grid(int rows, int H, int hkv, int R, int width, int page, int sms);
-long kv8_attention_work(int grid, int R, int hd);
+int kv8_attention_tile(int rows, int H, int hkv, int R, int hd);
+int kv8_attention_grid(int rows, int H, int hkv, int R, int width, int page, int hd, int sms);
+long kv8_attention_work(int grid, int tile, int R, int hd);
 int launch_kv8_attention(const Kv8Cache& c, const Kv8Attention& a, cudaStream_t st);
 
 // ----------------------------------------------------------------------- 4-bit weights (w4.cu)

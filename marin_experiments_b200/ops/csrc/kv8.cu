@@ -6,7 +6,8 @@
 // its 2^-6 .. 448 range, so a scale that is up to twice too large costs no precision, while a power
 // of two makes x / scale exact (one rounding in all, to the nearest code, ties to even) and lets the
 // scale of a page grow as tokens arrive: its older codes are multiplied by 2^-j, exact again but for
-// those that become subnormal. Values that are not finite are stored as e4m3's NaN.
+// those that become subnormal. Values that are not finite are stored as e4m3's NaN, and the sign of a
+// page's v_scale says that it holds one: the attention converts values without a look for NaN.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -38,15 +39,17 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// Largest finite magnitude of 8 bf16 values.
-__device__ __forceinline__ float amax8(const uint4& u) {
+// Largest finite magnitude of 8 bf16 values; `bad` if one is not finite.
+__device__ __forceinline__ float amax8(const uint4& u, bool& bad) {
   float a = 0.f;
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float lo = __uint_as_float((w[i] << 16) & 0x7fffffffu), hi = __uint_as_float(w[i] & 0x7fff0000u);
-    a = fmaxf(a, lo < INFINITY ? lo : 0.f);
-    a = fmaxf(a, hi < INFINITY ? hi : 0.f);
+    const bool lo_in = lo < INFINITY, hi_in = hi < INFINITY;
+    a = fmaxf(a, lo_in ? lo : 0.f);
+    a = fmaxf(a, hi_in ? hi : 0.f);
+    bad |= !(lo_in && hi_in);
   }
   return a;
 }
@@ -137,9 +140,10 @@ __global__ void __launch_bounds__(kAppendThreads)
     }
     const long base = ((long)page * c.hkv + head) * c.page * HD;
     float* sp = scales + (long)page * c.hkv + head;
-    const float old = off == 0 ? 0.f : *sp;
+    const float was = off == 0 ? 0.f : *sp, old = fabsf(was);
     const int step = together ? kAppendThreads : 32, me = together ? tid : lane;
     float amax = 0.f;
+    bool bad = false;
     uint4 held[kHeld];
     if (together) {
 #pragma unroll
@@ -149,18 +153,18 @@ __global__ void __launch_bounds__(kAppendThreads)
                               : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) amax = fmaxf(amax, amax8(held[i]));
+      for (int i = 0; i < kHeld; ++i) amax = fmaxf(amax, amax8(held[i], bad));
       amax = warp_max(amax);
       if (lane == 0) sh_max[warp] = amax;
-      __syncthreads();  // `together` is the same for the whole CTA
+      bad = __syncthreads_or(bad);  // `together` is the same for the whole CTA
 #pragma unroll
       for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, sh_max[w]);
       __syncthreads();
     } else {
       for (int p = me; p < n * LPT; p += 32)
-        amax = fmaxf(amax, amax8(*reinterpret_cast<const uint4*>(src + (r + p / LPT) * tok + (p % LPT) * 8)));
+        amax = fmaxf(amax, amax8(*reinterpret_cast<const uint4*>(src + (r + p / LPT) * tok + (p % LPT) * 8), bad));
       amax = warp_max(amax);
-      __syncwarp();
+      bad = __any_sync(0xffffffffu, bad);
     }
     const int need = need_exponent(amax);
     const float now = fmaxf(exp2_int(need), old);
@@ -180,7 +184,8 @@ __global__ void __launch_bounds__(kAppendThreads)
       for (int p = me; p < n * LPT; p += 32)
         dst[p] = codes8(*reinterpret_cast<const uint4*>(src + (r + p / LPT) * tok + (p % LPT) * 8), inv);
     }
-    if (me == 0) *sp = now;  // every thread has read `old` before the barrier above
+    // every thread has read `was` before the barrier above
+    if (me == 0) *sp = is_v && (bad || was < 0.f) ? -now : now;
   }
 }
 

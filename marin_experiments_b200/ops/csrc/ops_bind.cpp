@@ -691,13 +691,14 @@ Tensor kv8_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const 
   }
   if (T == 0) return o;
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const int grid = mxk::kv8_attention_grid((int)T, (int)H, c.hkv, (int)R, (int)tables.size(1), c.page, sms);
+  const int grid = mxk::kv8_attention_grid((int)T, (int)H, c.hkv, (int)R, (int)tables.size(1), c.page, c.hd, sms);
   need(grid > 0, "rows, heads and table width are beyond what one call indexes");
-  Tensor work = at::empty({mxk::kv8_attention_work(grid, (int)R, c.hd)}, ks.options());
+  const int tile = mxk::kv8_attention_tile((int)T, (int)H, c.hkv, (int)R, c.hd);
+  Tensor work = at::empty({mxk::kv8_attention_work(grid, tile, (int)R, c.hd)}, ks.options());
   mxk::Kv8Attention a{q.data_ptr(), qt, tables.data_ptr<int>(), lens.data_ptr<int>(),
                       starts.has_value() ? starts->data_ptr<int>() : nullptr, o.data_ptr(), (int)T, (int)H, (int)R,
                       (int)tables.size(1), starts.has_value() && !out.has_value(), (float)scale,
-                      work.data_ptr<float>(), grid};
+                      work.data_ptr<float>(), grid, tile};
   ok(mxk::launch_kv8_attention(c, a, stream()), "kv8_attention");
   return o;
 }

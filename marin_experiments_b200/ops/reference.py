@@ -395,7 +395,8 @@ def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, slots):
         n = 1
         while at + n < len(s) and off + n < page and s[at + n] == s[at] + n:
             n += 1
-        for x, cache, scale in ((k, k_cache, k_scale), (v, v_cache, v_scale)):
+        for x, cache, signed in ((k, k_cache, k_scale), (v, v_cache, v_scale)):
+            scale = signed.abs()
             y = x[at:at + n].float().transpose(0, 1)  # [heads, n, dim]
             fine = torch.isfinite(y)
             need = torch.exp2(kv8_exponent(torch.where(fine, y.abs(), torch.zeros_like(y)).amax((1, 2))).float())
@@ -405,7 +406,10 @@ def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, slots):
                 cache[pg, :, :off] = (cache[pg, :, :off].float() * ratio).to(cache.dtype)
             y = torch.where(fine, y / now[:, None, None], torch.full_like(y, float("nan")))
             cache[pg, :, off:off + n] = y.to(cache.dtype)
-            scale[pg] = now
+            if signed is v_scale:  # the sign marks pages that hold NaN
+                marked = ~fine.all(-1).all(-1) | ((signed[pg] < 0) & (off > 0))
+                now = torch.where(marked, -now, now)
+            signed[pg] = now
         at += n
 
 
@@ -427,7 +431,7 @@ def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, tables, lens, starts=No
             if m == 0:
                 o[i] = 0
                 continue
-            kk, vv = ((c[pg].float() * s[pg][..., None, None]).transpose(1, 2).reshape(-1, hkv, hd)[:m]
+            kk, vv = ((c[pg].float() * s[pg].abs()[..., None, None]).transpose(1, 2).reshape(-1, hkv, hd)[:m]
                       for c, s in ((k_cache, k_scale), (v_cache, v_scale)))
             sc = torch.einsum("grd,kgd->grk", q[i].float().view(hkv, h // hkv, hd), kk) * scale
             o[i] = torch.einsum("grk,kgd->grd", torch.softmax(sc, -1), vv).reshape(h, hd).to(q.dtype)

@@ -64,7 +64,7 @@ def attention64(q, c, starts=None, scale=None):
             if m <= 0:
                 continue
             pg = c["tables"][r, : -(-m // page)].long()
-            k, v = ((x[pg].double() * s[pg].double()[..., None, None]).transpose(1, 2).reshape(-1, hkv, hd)[:m]
+            k, v = ((x[pg].double() * s[pg].double().abs()[..., None, None]).transpose(1, 2).reshape(-1, hkv, hd)[:m]
                     for x, s in ((c["k"], c["ks"]), (c["v"], c["vs"])))
             for head in range(h):
                 kv = head // (h // hkv)

@@ -83,6 +83,12 @@ def test_append_keeps_what_is_not_finite_visible():
     got = c["k"].float() * c["ks"]
     assert torch.isnan(got).nonzero().tolist() == [[0, 0, 0, 0], [0, 0, 1, 1], [0, 0, 2, 2]]
     assert float(got[0, 0, 0, 1]) == 1.0
+    assert float(c["ks"]) > 0 and float(vs) < 0  # a page of values with NaN is marked
+    one = torch.ones(1, 1, 64).to(BF16)
+    api.kv8_append(one, one, c["k"], v, c["ks"], vs, ints([5]))
+    assert float(vs) < 0
+    api.kv8_append(one, one, c["k"], v, c["ks"], vs, ints([0]))  # the page begins anew
+    assert float(vs) > 0
 
 
 @pytest.mark.parametrize("lens,new", [([5, 0, 33], None), ([40, 0, 33, 70], [3, 0, 33, 1]), ([1, 20], [3, 2])])

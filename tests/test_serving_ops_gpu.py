@@ -265,12 +265,38 @@ def test_attention_nan_stays_with_the_rows_that_see_it(hd):
     k = c["k"].float()
     k[c["tables"][1, 2], 0, 4, 5] = float("nan")  # token 68 of the second request: a key
     c["v"], c["k"] = v.to(O.E4M3), k.to(O.E4M3)
+    c["vs"][c["tables"][0, 1]] *= -1  # as append marks it
     starts = [0, 6, 10]
     q = torch.randn(10, 3, hd, generator=torch.Generator().manual_seed(1)).to(BF16)
     want, size = O.attention64(q, c, starts)
     assert int(torch.isnan(want).sum()) == 3 * 3 + 2 * 3 * hd  # one column of rows 3..5; rows 8, 9
     got = attend(q.cuda(), cuda(c), starts=torch.tensor(starts, dtype=torch.int32, device="cuda"))
     O.close(got, want, O.attention_bound(want, size))
+
+
+@pytest.mark.parametrize("hd,n", [(64, 40), (128, 700)])
+def test_attention_of_appended_nan(hd, n):
+    """What is not finite in the appended rows reaches exactly the rows that see it, in decode and in
+    a call of several rows, in one CTA and in many."""
+    hkv, h, page = 2, 4, 64
+    pages = -(-n // page)
+    c = {"k": torch.zeros(pages, hkv, page, hd).to(O.E4M3), "ks": torch.zeros(pages, hkv)}
+    c |= {"v": c["k"].clone(), "vs": c["ks"].clone(), "tables": torch.arange(pages).int()[None].flip(1).contiguous(),
+          "lens": torch.tensor([n], dtype=torch.int32)}
+    g = torch.Generator().manual_seed(1)
+    k, v = torch.randn(n, hkv, hd, generator=g), torch.randn(n, hkv, hd, generator=g)
+    v[n - 3, 1, 7], v[5, 0, 9], v[5, 0, hd - 1] = float("inf"), float("nan"), float("-inf")
+    slots = torch.tensor([int(c["tables"][0, p // page]) * page + p % page for p in range(n)], dtype=torch.int32)
+    d = cuda(c)
+    api.kv8_append(k.to(BF16).cuda(), v.to(BF16).cuda(), d["k"], d["v"], d["ks"], d["vs"], slots.cuda())
+    c = {name: t.cpu() for name, t in d.items()}
+    for rows in (1, 5):
+        starts = [0, rows]
+        q = torch.randn(rows, h, hd, generator=g).to(BF16)
+        want, size = O.attention64(q, c, starts)
+        assert int(torch.isnan(want).sum()) == rows * 2 * 2 + min(rows, 3) * 2
+        got = attend(q.cuda(), d, starts=torch.tensor(starts, dtype=torch.int32, device="cuda"))
+        O.close(got, want, O.attention_bound(want, size))
 
 
 def test_attention_starts_that_do_not_ascend():
