@@ -205,14 +205,12 @@ struct Kv8Attention {
   int rows, H, R, width, zero_tail;
   float scale;
   float* work;  // kv8_attention_work floats
-  int grid;     // kv8_attention_grid
-  int tile;     // kv8_attention_tile
+  int grid, tile, cluster;  // of kv8_attention_plan
 };
-// CTAs of the attention for a call of these sizes (an upper bound on its work), or -1 if the sizes
-// are outside what it indexes; floats of its workspace.
-int kv8_attention_tile(int rows, int H, int hkv, int R, int hd);
-int kv8_attention_grid(int rows, int H, int hkv, int R, int width, int page, int hd, int sms);
-long kv8_attention_work(int grid, int tile, int R, int hd);
+// Sets how the call is split (grid, tile, cluster) from its sizes; false if they are beyond what it
+// indexes. Floats of its workspace.
+bool kv8_attention_plan(Kv8Attention& a, int hkv, int page, int hd, int sms);
+long kv8_attention_work(const Kv8Attention& a, int hd);
 int launch_kv8_attention(const Kv8Cache& c, const Kv8Attention& a, cudaStream_t st);
 
 // ----------------------------------------------------------------------- 4-bit weights (w4.cu)

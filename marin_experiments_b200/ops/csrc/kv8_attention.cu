@@ -14,22 +14,23 @@
 // 2^-12 of a weight at most (below 2^-29 of the largest weight: absolutely). Output sums are held in
 // units of the current page's scale; a page of another scale rescales them by a power of two.
 //
-// Conversion: cvt.f16x2.e4m3x2 runs on the XU pipe, 16 lanes a clock, which both products together
-// would keep busy for 80 % of the time that memory takes. Values are converted in the ALU instead:
-// the code's bits moved to f16's place are the value times 2^-8. That would turn a NaN code into a
-// number, so append marks pages that hold a NaN value in the sign of v_scale, and for those the rows
-// that see one are marked first. Keys keep the cvt, which keeps NaN.
+// A NaN value must reach the rows that see it and no other, but 0 * NaN would reach all rows of a
+// tile. append marks pages that hold a NaN value in the sign of v_scale; before such a page's values
+// are used, the outputs that see a NaN are marked and its codes are taken out.
 //
-// Split: all (request, row tile, kv head) segments are cut into steps of 128 keys, and the steps are
-// shared evenly among the CTAs, whatever the lengths. A segment that one CTA has whole is written at
-// once; else its CTAs write (max, sum, sum p v) and a second kernel, launched early so that its start
-// overlaps, joins them in order: results do not depend on timing, and no counter outlives a call.
+// Split, many segments (a segment: one request, row tile and kv head): segments are cut into steps of
+// 128 keys, and the steps are shared evenly among as many CTAs as the GPU holds, whatever the
+// lengths. A segment that one CTA has whole is written at once; else its CTAs write (max, sum,
+// sum p v) and a second kernel, launched early so that its start overlaps, joins them in order.
+// Few segments: a cluster of up to 8 CTAs takes one segment and joins through distributed shared
+// memory, one launch. Either way results do not depend on timing, and no counter outlives a call.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "kernels.h"
@@ -44,6 +45,7 @@ constexpr int kStep = kChunk * kWarps;
 constexpr int kMaxRequests = 4096;
 constexpr int kStages = 2;
 constexpr int kJoinWarps = 8;
+constexpr int kClusterSteps = 16;    // most steps a CTA of a cluster takes
 
 // CTAs an SM: what its registers hold without spilling (255 at two, 168 at three, 128 at four), and
 // at most what 228 KB of shared memory hold of rings (64 KB at hd 128, 32 KB at hd 64).
@@ -82,10 +84,12 @@ __device__ __forceinline__ uint32_t f16_hi(uint32_t w) {
   return d;
 }
 
-// Bytes 0 and 2 (lo) or 1 and 3 (hi) of w, e4m3 codes that are not NaN, as f16x2 of the value * 2^-8:
-// sign and eeeemmm go to f16's sign and the bits below its top exponent bit (bias 7 against 15).
-__device__ __forceinline__ uint32_t alu_lo(uint32_t w) { return ((w << 8) & 0x80008000u) | ((w << 7) & 0x3f803f80u); }
-__device__ __forceinline__ uint32_t alu_hi(uint32_t w) { return (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u); }
+// 2^x, 0 below 2^-126
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
@@ -124,7 +128,7 @@ __device__ __forceinline__ float group_sum(float v) {
 // saw no key has m = -inf and l = 0; one that met a NaN score keeps it.
 __device__ __forceinline__ float part_weight(float m, float l, float mx) {
   if (m == -INFINITY) return l == 0.f ? 0.f : 1.f;
-  return exp2f(m - mx);
+  return ex2(m - mx);
 }
 
 struct Work {
@@ -140,6 +144,30 @@ __host__ __device__ inline Work work_of(float* w, int grid, int tile, int hd) {
   return k;
 }
 
+// n / d for 0 <= n < 2^31, with mul = ceil(2^(31 + l) / d), l = ceil(log2 d): the product is off by
+// less than n * 2^l <= 2^(31 + l), one part in mul's scale.
+struct Div {
+  uint32_t mul;
+  int d, shift;
+  __device__ __forceinline__ int by(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n, mul) >> shift); }
+};
+Div make_div(int d) {
+  int l = 0;
+  while ((1LL << l) < d) ++l;
+  Div v;
+  v.d = d;
+  v.mul = d == 1 ? 0 : (uint32_t)(((1ULL << (31 + l)) + d - 1) / d);
+  v.shift = l - 1;
+  return v;
+}
+
+struct Args {
+  Kv8Cache c;
+  Kv8Attention a;
+  Div rep, hkv;    // query heads of a kv head; kv heads
+  int page_shift;
+};
+
 __device__ __forceinline__ int new_rows(const Kv8Attention& a, int r, int& first) {
   if (a.starts == nullptr) {
     first = r;
@@ -151,12 +179,11 @@ __device__ __forceinline__ int new_rows(const Kv8Attention& a, int r, int& first
   return n;
 }
 
-__device__ __forceinline__ int steps_of(const Kv8Attention& a, int page, int len) {
-  const long most = (long)a.width * page;
-  const long n = len < 0 ? 0 : (len > most ? most : len);
-  return n <= kStep ? 1 : (int)((n + kStep - 1) / kStep);
+__device__ __forceinline__ int steps_of(int cap, int len) {
+  return max(1, (int)(((unsigned)max(0, min(len, cap)) + kStep - 1) / kStep));
 }
 
+// First r with v[r + 1] > x, for ascending v[0 .. n].
 __device__ __forceinline__ int owner(const int* v, int n, int x) {
   int lo = 0, hi = n - 1;
   while (lo < hi) {
@@ -167,16 +194,61 @@ __device__ __forceinline__ int owner(const int* v, int n, int x) {
   return lo;
 }
 
-// First step of CTA i when `total` steps are shared among `grid` CTAs, and the CTA that has step x.
-__device__ __forceinline__ int share(int i, int total, int grid) { return (int)((long)i * total / grid); }
-__device__ __forceinline__ int cta_of(int x, int total, int grid) {
-  return (int)((((long)x + 1) * grid - 1) / total);
+// `total` steps among `used` <= total CTAs: the first total % used have one more.
+struct Share {
+  int per, more;
+  __device__ __forceinline__ Share(int total, int used) : per(total / used), more(total - per * used) {}
+  __device__ __forceinline__ int first(int cta) const { return cta * per + min(cta, more); }
+  __device__ __forceinline__ int cta(int step) const {
+    const int big = more * (per + 1);
+    return step < big ? step / (per + 1) : more + (step - big) / per;
+  }
+};
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_rank(const void* p, int rank) {  // the same place in another CTA
+  uint32_t d;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  return d;
+}
+__device__ __forceinline__ float ld_rank(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
+}
+template <int E>
+__device__ __forceinline__ void store_bf16(__nv_bfloat16* p, const float (&v)[E]) {
+  uint32_t u[E / 2];
+#pragma unroll
+  for (int e = 0; e < E; e += 2) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[e], v[e + 1]);
+    u[e / 2] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  if constexpr (E == 4) *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
+  else *reinterpret_cast<uint32_t*>(p) = u[0];
+}
+template <int E>
+__device__ __forceinline__ void load_f32(const float* p, float (&v)[E]) {
+  if constexpr (E == 4) {
+    const float4 u = *reinterpret_cast<const float4*>(p);
+    v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+  } else {
+    const float2 u = *reinterpret_cast<const float2*>(p);
+    v[0] = u.x; v[1] = u.y;
+  }
+}
+template <int E>
+__device__ __forceinline__ void store_f32(float* p, const float (&v)[E]) {
+  if constexpr (E == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
 }
 
 // Before the values of a page that holds NaN are used: marks the (row, dim) pairs that see a NaN of
 // this chunk, and zeroes the codes, which rows that do not see them would meet as 0 * NaN.
 template <int HD>
-__device__ __noinline__ void take_out_nan(uint8_t* values, uint8_t* marks, int lane, int key0, int rows, int rep,
+__device__ __noinline__ void take_out_nan(uint8_t* values, uint8_t* marks, int lane, int key0, int rows, Div rep,
                                           int row0, int pos0) {
   for (int i = lane; i < kChunk * HD; i += 32) {
     if ((values[i] & 0x7f) != 0x7f) continue;
@@ -185,20 +257,22 @@ __device__ __noinline__ void take_out_nan(uint8_t* values, uint8_t* marks, int l
     const int sw = HD == 128 ? ((key >> 1) & 3) << 1 : ((key >> 1) & 1) << 1;  // load's swizzle
     const int d = ((at / 16) ^ sw) * 16 + at % 16;
     for (int y = 0; y < rows; ++y)
-      if (key0 + key <= pos0 + (row0 + y) / rep) marks[y * HD + d] = 1;
+      if (key0 + key <= pos0 + rep.by(row0 + y)) marks[y * HD + d] = 1;
   }
 }
 
-// NQ: tiles of 8 rows that a segment's rows form.
-template <int HD, int NQ>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ))
-    attention_kernel(Kv8Cache c, Kv8Attention a) {
+// NQ: tiles of 8 rows that a segment's rows form. CLUSTER: one segment for each cluster.
+template <int HD, int NQ, bool CLUSTER>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ)) attention_kernel(const __grid_constant__ Args args) {
   constexpr int kRows = 8 * NQ;
   constexpr int KB = HD / 64;              // 16-byte pieces of a key a lane reads
   constexpr int MT = HD / 16;              // tiles of 16 dims of the output
+  constexpr int E = HD / 32;               // dims of an output row a lane joins
   constexpr int kStageBytes = 2 * kChunk * HD;
   constexpr int kLoads = kChunk * HD / 16 / 32;  // 16-byte copies a lane, keys or values
   constexpr int VW = HD / 32;              // words a lane reads of a value row
+  const Kv8Cache& c = args.c;
+  const Kv8Attention& a = args.a;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int warp_sums[kWarps];
   __shared__ float sh_m[kWarps][kRows], sh_l[kWarps][kRows];
@@ -207,47 +281,51 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ))
   int* prefix = reinterpret_cast<int*>(smem + kWarps * kStages * kStageBytes);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int rep = a.H / c.hkv;
+  const int rep = args.rep.d, cap = a.width << args.page_shift;
   const Work w = work_of(a.work, a.grid, kRows, HD);
   // the join's CTAs may take their places; they wait for this grid's end before they read
-  asm volatile("griddepcontrol.launch_dependents;");
+  if (!CLUSTER) asm volatile("griddepcontrol.launch_dependents;");
 
-  // Steps before each request. Ascending starts keep the sum below the host's bound; with any other
-  // nothing is computed.
+  // Steps (with CLUSTER segments) before each request, each thread's requests in a row. Ascending
+  // starts keep the sum below the host's bound; with any other nothing is computed.
+  const int per = (a.R + kThreads - 1) / kThreads;
+  auto weight = [&](int r, int& bad) {
+    int first;
+    const int n = new_rows(a, r, first);
+    if (a.starts != nullptr) bad |= a.starts[r + 1] < first;
+    return (n * rep + kRows - 1) / kRows * c.hkv * (CLUSTER ? 1 : steps_of(cap, a.lens[r]));
+  };
+  int mine = 0, bad = 0;
+  for (int i = 0; i < per; ++i)
+    if (tid * per + i < a.R) mine += weight(tid * per + i, bad);
   if (tid == 0) sh_any_nan = 0;
-  for (int x = tid; x < kRows * HD; x += kThreads) sh_nan[x] = 0;
-  int carry = 0, bad = 0;
-  for (int base = 0; base < a.R; base += kThreads) {
-    const int r = base + tid;
-    int v = 0, first;
-    if (r < a.R) {
-      const int n = new_rows(a, r, first);
-      if (a.starts != nullptr) bad |= a.starts[r + 1] < a.starts[r];
-      v = (n * rep + kRows - 1) / kRows * c.hkv * steps_of(a, c.page, a.lens[r]);
-    }
-    int x = v;
+  for (int x = tid; x < kRows * HD / 4; x += kThreads) reinterpret_cast<int*>(sh_nan)[x] = 0;
+  int x = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += u;
-    }
-    if (lane == 31) warp_sums[warp] = x;
-    __syncthreads();
-    int before = carry, all = carry;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      if (i < warp) before += warp_sums[i];
-      all += warp_sums[i];
-    }
-    if (r < a.R) prefix[r] = before + x - v;
-    carry = all;
-    __syncthreads();
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += u;
   }
-  if (tid == 0) prefix[a.R] = carry;
+  if (lane == 31) warp_sums[warp] = x;
   bad = __syncthreads_or(bad);
-  const int total = bad ? 0 : carry;
-  if (blockIdx.x == 0)
-    for (int r = tid; r <= a.R; r += kThreads) w.prefix[r] = r == a.R ? total : prefix[r];
+  int before = x - mine, total = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < warp) before += warp_sums[i];
+    total += warp_sums[i];
+  }
+  for (int i = 0; i < per; ++i) {
+    const int r = tid * per + i;
+    if (r < a.R) {
+      prefix[r] = before;
+      before += weight(r, bad);
+    }
+  }
+  if (bad) total = 0;
+  if (tid == 0) prefix[a.R] = total;
+  __syncthreads();
+  if (!CLUSTER && blockIdx.x == 0)
+    for (int r = tid; r <= a.R; r += kThreads) w.prefix[r] = prefix[r];
   if (a.zero_tail) {  // rows behind the last request
     const int last = max(0, min(a.rows, a.starts[a.R]));
     uint4* o = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (long)last * a.H * HD);
@@ -257,30 +335,37 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ))
   }
 
   const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(smem), ring = ring0 + warp * kStages * kStageBytes;
-  const int used = min(a.grid, total);  // so that every CTA that shares has a step
-  if ((int)blockIdx.x >= used) return;
-  const int end = share(blockIdx.x + 1, total, used);
-  int at = share(blockIdx.x, total, used);
+  int at, end;
+  const int parts = CLUSTER ? a.cluster : 1, rank = CLUSTER ? blockIdx.x % parts : 0;
+  if (CLUSTER) {
+    at = blockIdx.x / parts;
+    end = at < total ? at + 1 : at;  // the same for the whole cluster
+  } else {
+    const int used = min(a.grid, total);  // so that every CTA that shares has a step
+    if ((int)blockIdx.x >= used) return;
+    const Share sh(total, used);
+    at = sh.first(blockIdx.x);
+    end = sh.first(blockIdx.x + 1);
+  }
   const int begin = at;
   while (at < end) {
     const int r = owner(prefix, a.R, at);
     const int len_in = a.lens[r];
     int row0;
     const int n_new = new_rows(a, r, row0);
-    const int steps = steps_of(a, c.page, len_in);
-    const int in_r = at - prefix[r], seg = in_r / steps;  // segments of a request: row tiles x kv heads
-    const int s0 = in_r - seg * steps, seg_start = at - s0;
-    const int kh = seg % c.hkv, tile = seg / c.hkv;
-    const int s1 = min(steps, s0 + (end - at));
-    const int cap = a.width * c.page;
+    const int steps = steps_of(cap, len_in);
+    const int in_r = at - prefix[r], seg = CLUSTER ? in_r : in_r / steps;  // segments of a request: row tiles x kv heads
+    const int tile = args.hkv.by(seg), kh = seg - tile * c.hkv;
+    const int s0 = CLUSTER ? steps * rank / parts : in_r - seg * steps, seg_start = at - s0;
+    const int s1 = CLUSTER ? steps * (rank + 1) / parts : min(steps, s0 + (end - at));
     const bool too_long = len_in > cap;   // the table does not hold it: its rows become NaN
     const int len = max(0, min(len_in, cap));
     const int rows_here = min(kRows, n_new * rep - tile * kRows);
     const int pos0 = len_in - n_new;      // last position that new row 0 sees
 
     // this warp's chunks of the segment: first + kWarps * i, i < count
-    const int tile_last = pos0 + (tile * kRows + rows_here - 1) / rep;  // last position any row sees
-    const int tile_first = pos0 + tile * kRows / rep;                   // last position every row sees
+    const int tile_last = pos0 + args.rep.by(tile * kRows + rows_here - 1);  // last position any row sees
+    const int tile_first = pos0 + args.rep.by(tile * kRows);                   // last position every row sees
     const int seen = max(0, min(len, tile_last + 1));
     const int chunks = min(s1 * kWarps, (seen + kChunk - 1) / kChunk);
     const int first = s0 * kWarps + warp;
@@ -294,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ))
       ks_all = NAN;  // a page that the pool does not have: the rows that see it become NaN
       vs_all = 0.f;
       if (i < count) {
-        const int pg = table[(first + i * kWarps) * kChunk / c.page];
+        const int pg = table[(first + i * kWarps) * kChunk >> args.page_shift];
         if (pg >= 0 && pg < c.pages) {
           page_id = pg;
           ks_all = c.k_scale[(long)pg * c.hkv + kh];
@@ -309,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ))
       const int pg = __shfl_sync(0xffffffffu, page_id, i & 31);
       const uint32_t dst = ring + (i % kStages) * kStageBytes + (values ? kChunk * HD : 0);
       const uint8_t* src = (const uint8_t*)(values ? c.v : c.k) +
-                           (((long)max(pg, 0) * c.hkv + kh) * c.page + key0 % c.page) * HD;
+                           (((long)max(pg, 0) * c.hkv + kh) * c.page + (key0 & (c.page - 1))) * HD;
 #pragma unroll
       for (int x = 0; x < kLoads; ++x) {
         const int byte = (x * 32 + lane) * 16, key = byte / HD, col = byte % HD / 16;
@@ -321,6 +406,19 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ))
       }
       cp_commit();
     };
+    // Queries: lane (g, t) holds dims 64 b + 16 t .. + 15 of row g of each tile, four k steps of four
+    // dims, the order in which the lanes read the keys' codes (16 bytes at a time).
+    uint4 raw[NQ][2 * KB];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int y = 8 * n + g, x = tile * kRows + y, i = args.rep.by(x);
+      const __nv_bfloat16* p = (const __nv_bfloat16*)a.q + (row0 + i) * a.q_tok + (long)(kh * rep + x - i * rep) * HD + 16 * t;
+#pragma unroll
+      for (int b = 0; b < 2 * KB; ++b) {
+        raw[n][b] = make_uint4(0, 0, 0, 0);
+        if (y < rows_here) raw[n][b] = *reinterpret_cast<const uint4*>(p + 64 * (b / 2) + 8 * (b & 1));
+      }
+    }
     float ks_use = 0.f, vs_use = 0.f;
     if (count > 0) {
       fetch_pages(0);
@@ -338,23 +436,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ))
       }
     }
 
-    // Queries: lane (g, t) holds dims 64 b + 16 t .. + 15 of row g of each tile, four k steps of four
-    // dims, the order in which the lanes read the keys' codes (16 bytes at a time).
     uint32_t qf[NQ][4 * KB][2];
     float qs[NQ][2];  // of rows 2 t and 2 t + 1
     int pos[NQ][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      const int y = 8 * n + g, x = tile * kRows + y;
-      uint4 raw[2 * KB];
       float big = 0.f;
 #pragma unroll
       for (int b = 0; b < 2 * KB; ++b) {
-        raw[b] = make_uint4(0, 0, 0, 0);
-        if (y < rows_here)
-          raw[b] = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + (row0 + x / rep) * a.q_tok +
-                                                   (long)(kh * rep + x % rep) * HD + 64 * (b / 2) + 16 * t + 8 * (b & 1));
-        const uint32_t u[4] = {raw[b].x, raw[b].y, raw[b].z, raw[b].w};
+        const uint32_t u[4] = {raw[n][b].x, raw[n][b].y, raw[n][b].z, raw[n][b].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           big = fmaxf(big, fmaxf(fabsf(__uint_as_float(u[j] << 16)), fabsf(__uint_as_float(u[j] & 0xffff0000u))));
@@ -368,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ))
       const float back = __int_as_float((127 + e) << 23) * (a.scale * 1.4426950408889634f);
 #pragma unroll
       for (int b = 0; b < 2 * KB; ++b) {
-        const uint32_t u[4] = {raw[b].x, raw[b].y, raw[b].z, raw[b].w};
+        const uint32_t u[4] = {raw[n][b].x, raw[n][b].y, raw[n][b].z, raw[n][b].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           qf[n][2 * b + j / 2][j & 1] =
@@ -378,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ))
       for (int z = 0; z < 2; ++z) {
         const int yy = 8 * n + 2 * t + z;
         qs[n][z] = __shfl_sync(0xffffffffu, back, (2 * t + z) * 4);
-        pos[n][z] = yy < rows_here ? pos0 + (tile * kRows + yy) / rep : -1;
+        pos[n][z] = yy < rows_here ? pos0 + args.rep.by(tile * kRows + yy) : -1;
       }
     }
 
@@ -461,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ))
         for (int z = 0; z < 2; ++z) {
           const float mn = fmaxf(m[n][z], group_max(top[z]));
           const float ref = mn == -INFINITY ? 0.f : mn;
-          const float alpha = exp2f(m[n][z] - ref);
+          const float alpha = ex2(m[n][z] - ref);
           sub[z] = ref - 15.f;
           m[n][z] = mn;
           l[n][z] *= alpha;
@@ -473,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ))
           float p[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            p[x] = exp2f(s[h][n][x] - sub[x & 1]);
+            p[x] = ex2(s[h][n][x] - sub[x & 1]);
             l[n][x & 1] += p[x];
           }
           if (pscale != 1.f) {
@@ -497,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ))
       cp_wait<2 * kStages - 1>();  // the values of chunk i are there
       __syncwarp();
       if (vs < 0.f) {
-        take_out_nan<HD>(smem + (vb - ring0), sh_nan, lane, key0, rows_here, rep, tile * kRows, pos0);
+        take_out_nan<HD>(smem + (vb - ring0), sh_nan, lane, key0, rows_here, args.rep, tile * kRows, pos0);
         if (lane == 0) sh_any_nan = 1;
         __syncwarp();
       }
@@ -519,9 +609,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ))
         for (int x = 0; x < VW; ++x)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {  // two dims at a time: (key, dim), (key, dim + 1), (key + 1, dim), ..
-            const uint32_t p = __byte_perm(vw[0][x], vw[1][x], y ? 0x7632 : 0x5410);
-            const uint32_t q = __byte_perm(vw[2][x], vw[3][x], y ? 0x7632 : 0x5410);
-            const uint32_t a0 = alu_lo(p), a1 = alu_hi(p), a2 = alu_lo(q), a3 = alu_hi(q);
+            const uint32_t p = __byte_perm(vw[0][x], vw[1][x], y ? 0x7362 : 0x5140);
+            const uint32_t q = __byte_perm(vw[2][x], vw[3][x], y ? 0x7362 : 0x5140);
+            const uint32_t a0 = f16_lo(p), a1 = f16_hi(p), a2 = f16_lo(q), a3 = f16_hi(q);
 #pragma unroll
             for (int n = 0; n < NQ; ++n) mma(o[2 * x + y][n], a0, a1, a2, a3, pf[n][h][0], pf[n][h][1]);
           }
@@ -555,38 +645,83 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ))
 #pragma unroll
           for (int j = 0; j < MT; ++j)
             *reinterpret_cast<float2*>(so + y * HD + g * (HD / 8) + 2 * j) =
-                make_float2(o[j][n][z] * unit * 256.f, o[j][n][z + 2] * unit * 256.f);
+                make_float2(o[j][n][z] * unit, o[j][n][z + 2] * unit);
         }
       }
     __syncthreads();
     const bool whole = s0 == 0 && s1 == steps;
     const int slot = 2 * blockIdx.x + (seg_start >= begin ? 1 : 0);
-    for (int x = tid; x < rows_here * HD; x += kThreads) {
-      const int y = x / HD, d = x % HD;
-      float mx = -INFINITY, sum = 0.f, acc = 0.f;
+    // what a cluster's CTA has of the segment, behind the warps' parts
+    float* part = reinterpret_cast<float*>(smem) + kWarps * kRows * HD;
+    float* part_ml = part + kRows * HD;
+    auto out_row = [&](int y) {
+      const int x = tile * kRows + y, i = args.rep.by(x);
+      return (__nv_bfloat16*)a.out + ((long)(row0 + i) * a.H + kh * rep + x - i * rep) * HD + lane * E;
+    };
+    for (int y = warp; y < rows_here; y += kWarps) {
+      float mx = -INFINITY, sum = 0.f, acc[E];
 #pragma unroll
       for (int i = 0; i < kWarps; ++i) mx = fmaxf(mx, sh_m[i][y]);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = 0.f;
 #pragma unroll
       for (int i = 0; i < kWarps; ++i) {
         const float f = part_weight(sh_m[i][y], sh_l[i][y], mx);
         sum += sh_l[i][y] * f;
-        acc += reinterpret_cast<float*>(smem)[(i * kRows + y) * HD + d] * f;
+        float v[E];
+        load_f32(reinterpret_cast<float*>(smem) + (i * kRows + y) * HD + lane * E, v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += v[e] * f;
       }
-      if (sh_any_nan && sh_nan[x]) {
-        acc = NAN;
-        sh_nan[x] = 0;
+      if (sh_any_nan) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (sh_nan[y * HD + lane * E + e]) {
+            acc[e] = NAN;
+            sh_nan[y * HD + lane * E + e] = 0;
+          }
       }
       if (whole) {
-        const int xr = tile * kRows + y;
-        ((__nv_bfloat16*)a.out)[((long)(row0 + xr / rep) * a.H + kh * rep + xr % rep) * HD + d] =
-            __float2bfloat16(sum == 0.f ? 0.f : acc / sum);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = sum == 0.f ? 0.f : acc[e] * inv;
+        store_bf16(out_row(y), acc);
       } else {
-        w.acc[((long)slot * kRows + y) * HD + d] = acc;
-        if (d == 0) {
-          w.ml[(slot * kRows + y) * 2] = mx;
-          w.ml[(slot * kRows + y) * 2 + 1] = sum;
+        store_f32((CLUSTER ? part + y * HD : w.acc + ((long)slot * kRows + y) * HD) + lane * E, acc);
+        if (lane == 0) {
+          float* ml = CLUSTER ? part_ml + 2 * y : w.ml + (slot * kRows + y) * 2;
+          ml[0] = mx;
+          ml[1] = sum;
         }
       }
+    }
+    if constexpr (CLUSTER) {
+      if (parts > 1) {  // a segment has one CTA whole only if the others have none of it
+        const bool join = steps > 1;
+        if (join) {
+          cluster_sync();
+          for (int y = rank * kWarps + warp; y < rows_here; y += parts * kWarps) {
+            float mx = -INFINITY, sum = 0.f, acc[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = 0.f;
+            for (int i = 0; i < parts; ++i) mx = fmaxf(mx, ld_rank(in_rank(part_ml + 2 * y, i)));
+#pragma unroll 8
+            for (int i = 0; i < parts; ++i) {
+              const uint32_t ml = in_rank(part_ml + 2 * y, i), from = in_rank(part + y * HD + lane * E, i);
+              const float l = ld_rank(ml + 4), f = part_weight(ld_rank(ml), l, mx);
+              sum += l * f;
+#pragma unroll
+              for (int e = 0; e < E; ++e) acc[e] += ld_rank(from + 4 * e) * f;
+            }
+            const float inv = 1.f / sum;
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = sum == 0.f ? 0.f : acc[e] * inv;
+            store_bf16(out_row(y), acc);
+          }
+          cluster_sync();  // no CTA leaves while another reads its part
+        }
+      }
+      return;
     }
     __syncthreads();
     at += s1 - s0;
@@ -596,13 +731,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ))
 // Joins the segments that several CTAs shared: one CTA for each output row and head, whose warps
 // share the parts.
 template <int HD>
-__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(Kv8Cache c, Kv8Attention a) {
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ Args args) {
   constexpr int E = HD / 32;
+  const Kv8Cache& c = args.c;
+  const Kv8Attention& a = args.a;
   __shared__ float sh[kJoinWarps][HD], sh_m[kJoinWarps], sh_l[kJoinWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x / a.H, h = blockIdx.x % a.H;
   const Work w = work_of(a.work, a.grid, a.tile, HD);
-  const int rep = a.H / c.hkv;
+  const int rep = args.rep.d;
   // the caller's own inputs, complete before the attention kernel began
   int r = row;
   if (a.starts != nullptr) {
@@ -611,35 +748,33 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(Kv8Cache c, Kv8At
   }
   int row0;
   if (row - (a.starts ? a.starts[r] : r) >= new_rows(a, r, row0)) return;
-  const int steps = steps_of(a, c.page, a.lens[r]);
+  const int steps = steps_of(a.width << args.page_shift, a.lens[r]);
   if (steps == 1) return;  // one step has one CTA
-  const int x = (row - row0) * rep + h % rep, tile = x / a.tile, y = x % a.tile;
+  const int kh = args.rep.by(h), x = (row - row0) * rep + h - kh * rep, tile = x / a.tile, y = x % a.tile;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int total = w.prefix[a.R];
+  const int total = w.prefix[a.R], start = w.prefix[r];
   if (total == 0) return;
-  const int used = min(a.grid, total);
-  const int s0 = w.prefix[r] + (tile * c.hkv + h / rep) * steps;
-  const int c0 = cta_of(s0, total, used), c1 = cta_of(s0 + steps - 1, total, used);
+  const Share share(total, min(a.grid, total));
+  const int s0 = start + (tile * c.hkv + kh) * steps;
+  const int c0 = share.cta(s0), c1 = share.cta(s0 + steps - 1);
   if (c0 == c1) return;  // written by its CTA
   float mx = -INFINITY, sum = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll 2
+#pragma unroll 4
   for (int b = c0 + warp; b <= c1; b += kJoinWarps) {
     const int slot = (2 * b + (b == c0)) * a.tile + y;
-    const float m = w.ml[slot * 2], l = w.ml[slot * 2 + 1];
+    const float2 ml = *reinterpret_cast<const float2*>(w.ml + slot * 2);
     float v[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = w.acc[(long)slot * HD + e * 32 + lane];
-    const float mn = fmaxf(mx, m);
-    const float f0 = part_weight(mx, sum, mn), f1 = part_weight(m, l, mn);
-    sum = sum * f0 + l * f1;
+    load_f32(w.acc + (long)slot * HD + lane * E, v);
+    const float mn = fmaxf(mx, ml.x);
+    const float f0 = part_weight(mx, sum, mn), f1 = part_weight(ml.x, ml.y, mn);
+    sum = sum * f0 + ml.y * f1;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = acc[e] * f0 + v[e] * f1;
     mx = mn;
   }
-#pragma unroll
-  for (int e = 0; e < E; ++e) sh[warp][e * 32 + lane] = acc[e];
+  store_f32(sh[warp] + lane * E, acc);
   if (lane == 0) {
     sh_m[warp] = mx;
     sh_l[warp] = sum;
@@ -659,67 +794,96 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(Kv8Cache c, Kv8At
   ((__nv_bfloat16*)a.out)[((long)row * a.H + h) * HD + d] = __float2bfloat16(den == 0.f ? 0.f : num / den);
 }
 
-template <int HD, int NQ>
-int launch(const Kv8Cache& c, const Kv8Attention& a, cudaStream_t st) {
+template <int HD, int NQ, bool CLUSTER>
+int launch(const Args& args, cudaStream_t st) {
   constexpr int kRing = kWarps * kStages * 2 * kChunk * HD;
   static_assert(kWarps * 8 * NQ * HD * 4 <= kRing, "the join fits the ring");
+  static_assert(!CLUSTER || (kWarps + 1) * 8 * NQ * HD * 4 + 64 * NQ <= kRing, "so does a cluster's part");
+  const Kv8Attention& a = args.a;
   int dev = 0;
   cudaGetDevice(&dev);
   static std::atomic<bool> raised[64];
   if (dev < 0 || dev >= 64) return kErrBadArgsHost;
   if (!raised[dev].load()) {
-    if (cudaFuncSetAttribute(attention_kernel<HD, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(attention_kernel<HD, NQ, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              kRing + (kMaxRequests + 1) * 4) != cudaSuccess)
       return kErrBadArgsHost;
     raised[dev].store(true);
   }
-  count_launch();
-  attention_kernel<HD, NQ><<<a.grid, kThreads, kRing + (a.R + 1) * 4, st>>>(c, a);
   cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3((unsigned)a.grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kRing + (a.R + 1) * 4;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  count_launch();
+  if (CLUSTER) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = a.cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attention_kernel<HD, NQ, CLUSTER>, args) == cudaSuccess ? 0 : kErrBadArgsHost;
+  }
+  if (cudaLaunchKernelEx(&cfg, attention_kernel<HD, NQ, CLUSTER>, args) != cudaSuccess) return kErrBadArgsHost;
   cfg.gridDim = dim3((unsigned)(a.rows * a.H));
   cfg.blockDim = dim3(32 * kJoinWarps);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cfg.dynamicSmemBytes = 0;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
   cfg.numAttrs = 1;
   count_launch();
-  if (cudaLaunchKernelEx(&cfg, join_kernel<HD>, c, a) != cudaSuccess) return kErrBadArgsHost;
-  return cudaGetLastError() == cudaSuccess ? 0 : kErrBadArgsHost;
+  return cudaLaunchKernelEx(&cfg, join_kernel<HD>, args) == cudaSuccess ? 0 : kErrBadArgsHost;
 }
 
 }  // namespace
 
-// Rows of a tile: what a request's rows of one kv head need on average (8 in decode up to 8 query
-// heads a group), 16 at most at hd 128 and 32 at hd 64, where the registers end.
-int kv8_attention_tile(int rows, int H, int hkv, int R, int hd) {
-  const long n = R < 1 || hkv < 1 ? 1 : ((long)rows + R - 1) / R * (H / hkv);
-  return n <= 8 ? 8 : (n <= 16 || hd == 128 ? 16 : 32);
+bool kv8_attention_plan(Kv8Attention& a, int hkv, int page, int hd, int sms) {
+  if (a.R < 1 || a.R > kMaxRequests || a.rows < 0 || hkv < 1 || a.H % hkv) return false;
+  if ((long)a.width * page > 0x7fffffffL || (long)a.rows * a.H > 0x7fffffffL) return false;
+  // Rows of a tile: what a request's rows of one kv head need on average (8 in decode up to 8 query
+  // heads a group), 16 at most at hd 128 and 32 at hd 64, where the registers end.
+  const long n = ((long)a.rows + a.R - 1) / a.R * (a.H / hkv);
+  a.tile = n <= 8 ? 8 : (n <= 16 || hd == 128 ? 16 : 32);
+  const long tiles = ((long)a.rows * (a.H / hkv) + a.tile - 1) / a.tile + a.R;  // each request rounds up at most once
+  const long steps = std::max(1L, ((long)a.width * page + kStep - 1) / kStep);
+  const long segs = a.starts == nullptr ? (long)a.R * hkv * ((a.H / hkv + a.tile - 1) / a.tile) : tiles * hkv;
+  if ((double)tiles * hkv * steps > 2.0e9) return false;
+  const long ctas = (long)sms * ctas_per_sm(hd, a.tile);
+  a.cluster = 0;
+  int size = 8;
+  while (size > 1 && segs * size > ctas) size /= 2;
+  while (size > 1 && size / 2 >= steps) size /= 2;
+  if (a.tile <= 16 && segs * size <= ctas && steps <= (long)kClusterSteps * size) {
+    a.cluster = size;
+    a.grid = (int)(segs * size);
+  } else {
+    a.grid = (int)std::min(tiles * hkv * steps, ctas);
+  }
+  return true;
 }
 
-int kv8_attention_grid(int rows, int H, int hkv, int R, int width, int page, int hd, int sms) {
-  if (R < 1 || R > kMaxRequests || rows < 0 || hkv < 1 || H % hkv || (long)width * page > 0x7fffffffL) return -1;
-  if ((long)rows * H > 0x7fffffffL) return -1;
-  const int tile = kv8_attention_tile(rows, H, hkv, R, hd);
-  const long tiles = ((long)rows * (H / hkv) + tile - 1) / tile + R;  // each request rounds up at most once
-  const long steps = ((long)width * page + kStep - 1) / kStep;
-  if ((double)tiles * hkv * (steps < 1 ? 1 : steps) > 2.0e9) return -1;
-  const long most = tiles * hkv * (steps < 1 ? 1 : steps);
-  const long ctas = (long)sms * ctas_per_sm(hd, tile);
-  return (int)(most < ctas ? (most < 1 ? 1 : most) : ctas);
+long kv8_attention_work(const Kv8Attention& a, int hd) {
+  return a.cluster ? 0 : 2L * a.grid * a.tile * (hd + 2) + a.R + 1;
 }
-
-long kv8_attention_work(int grid, int tile, int R, int hd) { return 2L * grid * tile * (hd + 2) + R + 1; }
 
 int launch_kv8_attention(const Kv8Cache& c, const Kv8Attention& a, cudaStream_t st) {
   if (a.rows < 1) return 0;
-  if (c.page % kChunk || a.grid < 1) return kErrBadArgsHost;
-  if (c.hd == 64 && a.tile == 8) return launch<64, 1>(c, a, st);
-  if (c.hd == 64 && a.tile == 16) return launch<64, 2>(c, a, st);
-  if (c.hd == 64 && a.tile == 32) return launch<64, 4>(c, a, st);
-  if (c.hd == 128 && a.tile == 8) return launch<128, 1>(c, a, st);
-  if (c.hd == 128 && a.tile == 16) return launch<128, 2>(c, a, st);
+  if (c.page % kChunk || (c.page & (c.page - 1)) || a.grid < 1) return kErrBadArgsHost;
+  Args args{c, a, make_div(a.H / c.hkv), make_div(c.hkv), 0};
+  while ((1 << args.page_shift) < c.page) ++args.page_shift;
+  if (a.cluster) {
+    if (c.hd == 64 && a.tile == 8) return launch<64, 1, true>(args, st);
+    if (c.hd == 64 && a.tile == 16) return launch<64, 2, true>(args, st);
+    if (c.hd == 128 && a.tile == 8) return launch<128, 1, true>(args, st);
+    if (c.hd == 128 && a.tile == 16) return launch<128, 2, true>(args, st);
+    return kErrBadArgsHost;
+  }
+  if (c.hd == 64 && a.tile == 8) return launch<64, 1, false>(args, st);
+  if (c.hd == 64 && a.tile == 16) return launch<64, 2, false>(args, st);
+  if (c.hd == 64 && a.tile == 32) return launch<64, 4, false>(args, st);
+  if (c.hd == 128 && a.tile == 8) return launch<128, 1, false>(args, st);
+  if (c.hd == 128 && a.tile == 16) return launch<128, 2, false>(args, st);
   return kErrBadArgsHost;
 }
 

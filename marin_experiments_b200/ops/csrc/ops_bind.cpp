@@ -690,15 +690,17 @@ Tensor kv8_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const 
     o = at::empty(q.sizes(), q.options());
   }
   if (T == 0) return o;
-  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const int grid = mxk::kv8_attention_grid((int)T, (int)H, c.hkv, (int)R, (int)tables.size(1), c.page, c.hd, sms);
-  need(grid > 0, "rows, heads and table width are beyond what one call indexes");
-  const int tile = mxk::kv8_attention_tile((int)T, (int)H, c.hkv, (int)R, c.hd);
-  Tensor work = at::empty({mxk::kv8_attention_work(grid, tile, (int)R, c.hd)}, ks.options());
   mxk::Kv8Attention a{q.data_ptr(), qt, tables.data_ptr<int>(), lens.data_ptr<int>(),
                       starts.has_value() ? starts->data_ptr<int>() : nullptr, o.data_ptr(), (int)T, (int)H, (int)R,
-                      (int)tables.size(1), starts.has_value() && !out.has_value(), (float)scale,
-                      work.data_ptr<float>(), grid, tile};
+                      (int)tables.size(1), starts.has_value() && !out.has_value(), (float)scale};
+  need(mxk::kv8_attention_plan(a, c.hkv, c.page, c.hd, at::cuda::getCurrentDeviceProperties()->multiProcessorCount),
+       "rows, heads and table width are beyond what one call indexes");
+  const long floats = mxk::kv8_attention_work(a, c.hd);
+  Tensor work;
+  if (floats) {
+    work = at::empty({floats}, ks.options());
+    a.work = work.data_ptr<float>();
+  }
   ok(mxk::launch_kv8_attention(c, a, stream()), "kv8_attention");
   return o;
 }

@@ -185,7 +185,8 @@ def test_attention_decode(hd, h, hkv, page, lens):
 
 
 @pytest.mark.parametrize("lens,h,hkv,hd", [([9000], 8, 1, 128), ([4097, 20000], 4, 2, 64), ([50] * 200, 4, 2, 128),
-                                           ([1] * 700, 2, 1, 64)])
+                                           ([1] * 700, 2, 1, 64), ([1500, 129, 40] * 20 + [9000], 4, 2, 128),
+                                           ([700] * 130 + [20000], 2, 1, 64)])
 def test_attention_splits(lens, h, hkv, hd):
     """Few long requests (many CTAs a segment) and many short ones (many segments a CTA)."""
     c = O.make_cache(lens, hkv=hkv, hd=hd, page=64, seed=1)
