@@ -205,7 +205,7 @@ struct Kv8Attention {
   int rows, H, R, width, zero_tail;
   float scale;
   float* work;  // kv8_attention_work floats
-  int grid, tile, cluster;  // of kv8_attention_plan
+  int grid, resident, tile, cluster;  // of kv8_attention_plan
 };
 // Sets how the call is split (grid, tile, cluster) from its sizes; false if they are beyond what it
 // indexes. Floats of its workspace.
@@ -215,7 +215,8 @@ int launch_kv8_attention(const Kv8Cache& c, const Kv8Attention& a, cudaStream_t 
 
 // ----------------------------------------------------------------------- 4-bit weights (w4.cu)
 int launch_linear_w4(const void* x, long x_tok, const void* codes, const void* scales, const void* residual, long r_tok,
-                     void* out, int T, int N, int K, int group, int glu, cudaStream_t st);
+                     void* out, int T, int N, int K, int group, int glu, int sms, float* work, cudaStream_t st);
+long linear_w4_work(int T, int N, int K, int sms);  // floats of its workspace
 int launch_dequant_w4(const void* codes, const void* scales, void* out, int N, int K, int group, cudaStream_t st);
 
 // ------------------------------------------------------------------- hashed n-gram embedding (ngram.cu)

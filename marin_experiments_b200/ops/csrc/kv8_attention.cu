@@ -45,6 +45,11 @@ constexpr int kStep = kChunk * kWarps;
 constexpr int kMaxRequests = 4096;
 constexpr int kStages = 2;
 constexpr int kJoinWarps = 8;
+// Long calls make up to kRounds CTAs for each that runs at once, of kManySteps steps or more: SMs are
+// not equally fast, and the hardware gives the next CTA to the one that is free (48 requests of up to
+// 32768 tokens: 254 us at 1 round, 249 at 2, 242 at 4, 237 at 8; 259 with 8 steps a CTA).
+constexpr long kRounds = 8;
+constexpr int kManySteps = 16;
 constexpr int kClusterSteps = 16;    // most steps a CTA of a cluster takes
 
 // CTAs an SM: what its registers hold without spilling (255 at two, 168 at three, 128 at four), and
@@ -194,6 +199,12 @@ __device__ __forceinline__ int owner(const int* v, int n, int x) {
   return lo;
 }
 
+// CTAs that share the steps: all that the GPU holds at once, each with one step at least, and up to
+// the grid's multiple of that where each still has kManySteps.
+__device__ __forceinline__ int used_ctas(const Kv8Attention& a, int total) {
+  return min(total, max(a.resident, min(a.grid, total / kManySteps)));
+}
+
 // `total` steps among `used` <= total CTAs: the first total % used have one more.
 struct Share {
   int per, more;
@@ -341,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ)) attention_k
     at = blockIdx.x / parts;
     end = at < total ? at + 1 : at;  // the same for the whole cluster
   } else {
-    const int used = min(a.grid, total);  // so that every CTA that shares has a step
+    const int used = used_ctas(a, total);
     if ((int)blockIdx.x >= used) return;
     const Share sh(total, used);
     at = sh.first(blockIdx.x);
@@ -497,10 +508,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ)) attention_k
       float s[2][NQ][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        float s2[NQ][4];  // every other k step: chains of dependent products half as long
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) s[h][n][x] = 0.f;
+          for (int x = 0; x < 4; ++x) s[h][n][x] = s2[n][x] = 0.f;
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
           const int key = 16 * h + g, col = 4 * b + t;
@@ -511,9 +523,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ)) attention_k
           for (int j = 0; j < 4; ++j) {
             const uint32_t a0 = f16_lo(uw[j]), a1 = f16_lo(vw[j]), a2 = f16_hi(uw[j]), a3 = f16_hi(vw[j]);
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) mma(s[h][n], a0, a1, a2, a3, qf[n][4 * b + j][0], qf[n][4 * b + j][1]);
+            for (int n = 0; n < NQ; ++n)
+              mma(j & 1 ? s2[n] : s[h][n], a0, a1, a2, a3, qf[n][4 * b + j][0], qf[n][4 * b + j][1]);
           }
         }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[h][n][x] += s2[n][x];
       }
       __syncwarp();  // all lanes have read the keys: their place takes those of the chunk after next
       if (nx < count) {
@@ -754,7 +771,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int total = w.prefix[a.R], start = w.prefix[r];
   if (total == 0) return;
-  const Share share(total, min(a.grid, total));
+  const Share share(total, used_ctas(a, total));
   const int s0 = start + (tile * c.hkv + kh) * steps;
   const int c0 = share.cta(s0), c1 = share.cta(s0 + steps - 1);
   if (c0 == c1) return;  // written by its CTA
@@ -858,7 +875,9 @@ bool kv8_attention_plan(Kv8Attention& a, int hkv, int page, int hd, int sms) {
     a.cluster = size;
     a.grid = (int)(segs * size);
   } else {
-    a.grid = (int)std::min(tiles * hkv * steps, ctas);
+    const long most = tiles * hkv * steps;
+    a.resident = (int)std::min(most, ctas);
+    a.grid = (int)std::max<long>(a.resident, std::min(kRounds * ctas, most / kManySteps));
   }
   return true;
 }

@@ -742,9 +742,13 @@ Tensor linear_w4(const Tensor& x, const Tensor& codes, const Tensor& scales, con
     need(residual->size(0) == x.size(0), "one residual row for each row of x");
   }
   c10::cuda::CUDAGuard g(codes.device());
-  Tensor out = at::empty({x.size(0), glu ? N / 2 : N}, x.options());
+  Tensor out = at::empty({x.size(0), glu ? N / 2 : N}, x.options()), work;
+  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const long floats = mxk::linear_w4_work((int)x.size(0), (int)N, (int)K, sms);
+  if (floats) work = at::empty({floats}, x.options().dtype(at::kFloat));
   ok(mxk::launch_linear_w4(x.data_ptr(), xt, codes.data_ptr(), scales.data_ptr(), ptr<const void>(residual), rt,
-                           out.data_ptr(), (int)x.size(0), (int)N, (int)K, group, glu, stream()),
+                           out.data_ptr(), (int)x.size(0), (int)N, (int)K, group, glu, sms,
+                           floats ? work.data_ptr<float>() : nullptr, stream()),
      "linear_w4");
   return out;
 }

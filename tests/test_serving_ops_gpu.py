@@ -323,7 +323,8 @@ def w4_case(n, k, group, t, seed=0):
 
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("n,k,t", [(1, 128, 1), (17, 128, 3), (64, 1152, 8), (100, 2048, 9), (33, 4224, 16),
-                                   (16, 256, 31), (250, 384, 33), (40, 1024, 64)])
+                                   (16, 256, 31), (250, 384, 33), (40, 1024, 64),
+                                     (5000, 256, 5), (70, 12288, 33), (33, 14336, 64), (20, 98304, 3)])
 def test_linear_w4(n, k, t, group):
     codes, packed, scales, x = w4_case(n, k, group, t)
     y, size = O.w4_64(x, codes, scales)
