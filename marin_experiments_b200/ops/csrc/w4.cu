@@ -242,9 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
   // launched early: the kernel before may still be writing x (or the weights)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (a.slices > 1) asm volatile("griddepcontrol.launch_dependents;");
-  Scales<BU, GW> s_ring[kStages][2];
-#pragma unroll
-  for (int i = 0; i < kStages; ++i) fetch(s_ring[i]);
+  // x before the weights, which would keep the memory busy for longer than it waits.
   // Blocks that the last unit lacks meet zeros (their codes are what the ring held).
   for (int c = tid; c < units * BU * 16; c += kThreads) {
     const __nv_bfloat16* from = a.x + b0 * 128 + c * 8;
@@ -257,10 +255,13 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
     }
   }
   cp_commit();
+  Scales<BU, GW> s_ring[kStages][2];
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) fetch(s_ring[i]);
   const __nv_bfloat16* xp[NT];  // columns past T repeat the last row and are not stored
 #pragma unroll
   for (int n = 0; n < NT; ++n) xp[n] = xs + min(n * 8 + g, a.T - 1) * x_pitch + t * 8;
-  cp_wait<0>();
+  cp_wait<kStages>();
   __syncthreads();
 
   // in registers, so that the conversions take them as operands
