@@ -32,7 +32,7 @@ namespace {
 constexpr int kWarps = 16;
 constexpr int kStages = 2;  // units of a warp on their way
 // Blocks of 128 values of K in a unit: 256 bytes of a row, or 128 where x needs the shared memory.
-__host__ __device__ constexpr int blocks_of(int nt) { return nt <= 2 ? 4 : 2; }
+__host__ __device__ constexpr int blocks_of(int nt) { return nt == 1 ? 4 : 2; }
 constexpr int kMaxSmem = 226 * 1024;  // of 227 KB; part_tile is static
 constexpr double kSliceCost = 0.1;  // of one more slice, in units
 constexpr int kThreads = kWarps * 32;
