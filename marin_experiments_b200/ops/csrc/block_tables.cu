@@ -16,6 +16,7 @@
 #include <stdint.h>
 
 #include "kernels.h"
+#include "pdl.cuh"
 
 namespace mxk {
 namespace {
@@ -83,6 +84,7 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ int bad_any;
   const int tid = threadIdx.x;
   if (tid == 0) bad_any = 0;
+  wait_for_previous();
   const int count = *free_count;
   int bad = count < 0 || count > capacity ? kTablesBadInput : 0;
   long long sum_new = 0, sum_more = 0;
@@ -169,6 +171,7 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ int bad_any;
   const int tid = threadIdx.x;
   if (tid == 0) bad_any = 0;
+  wait_for_previous();
   const int count = *free_count;
   int bad = count < 0 || count > capacity ? kTablesBadInput : 0;
   long long total = 0;
@@ -215,19 +218,21 @@ int launch_block_tables_extend(int* tables, int width, const int* lens, const in
   if (grid < 1) grid = 1;
   if (grid > 148) grid = 148;
   count_launch();
-  extend_kernel<<<grid, kThreads, 2 * (R + 1) * sizeof(int), st>>>(tables, width, lens, grow, R, free_pages, capacity,
-                                                                   free_count, page, rows, lens_out, count_out, starts,
-                                                                   slots, requests, positions, status);
-  return cudaGetLastError() == cudaSuccess ? 0 : kErrBadArgsHost;
+  return launch_early(extend_kernel, dim3(grid), kThreads, 2 * (R + 1) * sizeof(int), st, 1, tables, width, lens, grow, R,
+                      free_pages, capacity, free_count, page, rows, lens_out, count_out, starts, slots, requests,
+                      positions, status) == cudaSuccess
+             ? 0
+             : kErrBadArgsHost;
 }
 
 int launch_block_tables_release(int* tables, int width, int* lens, const uint8_t* done, int R, int* free_pages,
                                 int capacity, int* free_count, int page, int* status, cudaStream_t st) {
   if (R < 1 || R > kTablesMaxRequests || page < 1 || width < 0) return kErrBadArgsHost;
   count_launch();
-  release_kernel<<<1, kThreads, (R + 1) * sizeof(int), st>>>(tables, width, lens, done, R, free_pages, capacity,
-                                                             free_count, page, status);
-  return cudaGetLastError() == cudaSuccess ? 0 : kErrBadArgsHost;
+  return launch_early(release_kernel, dim3(1), kThreads, (R + 1) * sizeof(int), st, 1, tables, width, lens, done, R,
+                      free_pages, capacity, free_count, page, status) == cudaSuccess
+             ? 0
+             : kErrBadArgsHost;
 }
 
 }  // namespace mxk

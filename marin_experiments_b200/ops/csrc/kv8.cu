@@ -16,6 +16,7 @@
 #include <stdint.h>
 
 #include "kernels.h"
+#include "pdl.cuh"
 
 namespace mxk {
 namespace {
@@ -33,37 +34,37 @@ __device__ __forceinline__ int need_exponent(float amax) {
   return min(kMaxExp, max(kMinExp, e));
 }
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+// Largest magnitudes of the low and the high halves of 8 bf16 values, two 16-bit numbers (0x7f80 and
+// above: not finite); `most` before.
+__device__ __forceinline__ uint32_t amax8(const uint4& u, uint32_t most) {
+  most = __vmaxu2(most, u.x & 0x7fff7fffu);
+  most = __vmaxu2(most, u.y & 0x7fff7fffu);
+  most = __vmaxu2(most, u.z & 0x7fff7fffu);
+  return __vmaxu2(most, u.w & 0x7fff7fffu);
 }
-
-// Largest finite magnitude of 8 bf16 values; `bad` if one is not finite.
-__device__ __forceinline__ float amax8(const uint4& u, bool& bad) {
-  float a = 0.f;
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// The same of the finite ones alone.
+__device__ __forceinline__ uint32_t finite8(uint4 u, uint32_t most) {
+  uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float lo = __uint_as_float((w[i] << 16) & 0x7fffffffu), hi = __uint_as_float(w[i] & 0x7fff0000u);
-    const bool lo_in = lo < INFINITY, hi_in = hi < INFINITY;
-    a = fmaxf(a, lo_in ? lo : 0.f);
-    a = fmaxf(a, hi_in ? hi : 0.f);
-    bad |= !(lo_in && hi_in);
+    if ((w[i] & 0x7f80u) == 0x7f80u) w[i] &= 0xffff0000u;
+    if ((w[i] & 0x7f800000u) == 0x7f800000u) w[i] &= 0xffffu;
   }
-  return a;
+  return amax8(make_uint4(w[0], w[1], w[2], w[3]), most);
 }
 
 __device__ __forceinline__ float or_nan(float x) { return fabsf(x) < INFINITY ? x : NAN; }
 
-// 8 bf16 values times inv, as 8 codes.
+// 8 bf16 values times inv, as 8 codes. CHECK: what is not finite becomes NaN.
+template <bool CHECK>
 __device__ __forceinline__ uint2 codes8(const uint4& u, float inv) {
   uint32_t w[4] = {u.x, u.y, u.z, u.w}, c[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float2 f;
-    f.x = or_nan(__uint_as_float(w[i] << 16)) * inv;
-    f.y = or_nan(__uint_as_float(w[i] & 0xffff0000u)) * inv;
+    float2 f = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    if (CHECK) f = make_float2(or_nan(f.x), or_nan(f.y));
+    f.x *= inv;
+    f.y *= inv;
     c[i] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
   }
   return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
@@ -95,16 +96,20 @@ __device__ __forceinline__ uint2 rescale8(uint2 u, float ratio) {
 // rows, one head, keys or values. Few runs start in a window of prompt tokens: the CTA takes each
 // together, with the run's values in registers between the maximum and the rounding (one read). Many
 // start in a window of decode tokens: each warp takes its own.
+//
+// What bounds it: in prompts the bytes, 2 in and 1 out a value; in decode two dependent loads. A run's
+// values are loaded while its length is still looked for (they are masked when it is known).
 constexpr int kAppendThreads = 256;
-constexpr int kMaxPage = 128;
+constexpr int kAppendWarps = kAppendThreads / 32;
 
-template <int HD>
+template <int HD, int PAGE>
 __global__ void __launch_bounds__(kAppendThreads)
-    append_kernel(Kv8Cache c, const __nv_bfloat16* __restrict__ k_new, const __nv_bfloat16* __restrict__ v_new,
-                  long k_tok, long v_tok, const int* __restrict__ slots, int rows, int window) {
-  constexpr int LPT = HD / 8;                        // lanes a token (8 values each)
-  constexpr int kHeld = kMaxPage * HD / 8 / kAppendThreads;  // 16-byte pieces a thread holds of a full run
-  __shared__ float sh_max[kAppendThreads / 32];
+    append_kernel(const __grid_constant__ Kv8Cache c, const __nv_bfloat16* __restrict__ k_new,
+                  const __nv_bfloat16* __restrict__ v_new, long k_tok, long v_tok, const int* __restrict__ slots,
+                  int rows, int window) {
+  constexpr int LPT = HD / 8;  // 16-byte pieces of a row
+  constexpr int kHeld = (PAGE * LPT + kAppendThreads - 1) / kAppendThreads;  // that a thread holds of a full run
+  __shared__ uint32_t sh_max[kAppendWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int head = blockIdx.y;
   const bool is_v = blockIdx.z;
@@ -112,81 +117,104 @@ __global__ void __launch_bounds__(kAppendThreads)
   const long tok = is_v ? v_tok : k_tok;
   uint8_t* cache = (uint8_t*)(is_v ? c.v : c.k);
   float* scales = is_v ? c.v_scale : c.k_scale;
-  const int r0 = blockIdx.x * window, row = r0 + lane;
-  const int limit = c.pages * c.page;  // below 2^31 by the host's check
-  // runs that start in this window
-  int slot = -1, prev = -2;
-  if (lane < window && row < rows) {
-    slot = slots[row];
-    if (row > 0) prev = slots[row - 1];
-  }
-  const bool first = slot >= 0 && slot < limit && (slot % c.page == 0 || prev != slot - 1);
-  const uint32_t runs = __ballot_sync(0xffffffffu, first);
-  const bool together = __popc(runs) <= 2;
-  int index = 0;
-  for (uint32_t left = runs; left; left &= left - 1, ++index) {
-    if (!together && (index % (kAppendThreads / 32)) != warp) continue;
-    const int l = __ffs(left) - 1;
-    const int s0 = __shfl_sync(0xffffffffu, slot, l);
-    const int page = s0 / c.page, off = s0 % c.page, r = r0 + l;
-    // length of the run: to the end of the page, the rows or the sequence of slots
-    const int most = min(c.page - off, rows - r);
-    int n = 0;
-    for (int b = 0; b < most; b += 32) {
-      const bool in = b + lane < most && slots[r + b + lane] == s0 + b + lane;
-      const uint32_t m = __ballot_sync(0xffffffffu, in);
-      n += m == 0xffffffffu ? 32 : __ffs(~m) - 1;
-      if (m != 0xffffffffu) break;
+  const int limit = c.pages * PAGE;  // below 2^31 by the host's check
+  wait_for_previous();
+  for (int r0 = blockIdx.x * window; r0 < min(rows, (int)(blockIdx.x + 1) * window); r0 += 32) {
+    const int row = r0 + lane;
+    // runs that start in these 32 rows
+    int slot = -1, prev = -2;
+    if (row < min(rows, (int)(blockIdx.x + 1) * window)) {
+      slot = slots[row];
+      if (row > 0) prev = slots[row - 1];
     }
-    const long base = ((long)page * c.hkv + head) * c.page * HD;
-    float* sp = scales + (long)page * c.hkv + head;
-    const float was = off == 0 ? 0.f : *sp, old = fabsf(was);
-    const int step = together ? kAppendThreads : 32, me = together ? tid : lane;
-    float amax = 0.f;
-    bool bad = false;
-    uint4 held[kHeld];
-    if (together) {
+    const bool first = slot >= 0 && slot < limit && (slot % PAGE == 0 || prev != slot - 1);
+    const uint32_t runs = __ballot_sync(0xffffffffu, first);
+    const bool together = __popc(runs) <= 2;
+    int index = 0;
+    for (uint32_t left = runs; left; left &= left - 1, ++index) {
+      if (!together && (index % kAppendWarps) != warp) continue;
+      const int l = __ffs(left) - 1;
+      const int s0 = __shfl_sync(0xffffffffu, slot, l);
+      const int page = s0 / PAGE, off = s0 % PAGE, r = r0 + l;
+      const int most = min(PAGE - off, rows - r);  // rows that the run may have
+      const long base = ((long)page * c.hkv + head) * PAGE * HD;
+      float* sp = scales + (long)page * c.hkv + head;
+      const float was = off == 0 ? 0.f : *sp, old = fabsf(was);
+      auto piece = [&](int p) { return *reinterpret_cast<const uint4*>(src + (r + p / LPT) * tok + (p % LPT) * 8); };
+      uint4 held[kHeld];
+      if (together) {
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
-        const int p = me + i * kAppendThreads;
-        held[i] = p < n * LPT ? *reinterpret_cast<const uint4*>(src + (r + p / LPT) * tok + (p % LPT) * 8)
-                              : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kHeld; ++i) {
+          const int p = tid + i * kAppendThreads;
+          held[i] = p < most * LPT ? piece(p) : make_uint4(0, 0, 0, 0);
+        }
       }
+      int n = 0;  // rows that it has
+      bool on = true;
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) amax = fmaxf(amax, amax8(held[i], bad));
-      amax = warp_max(amax);
-      if (lane == 0) sh_max[warp] = amax;
-      bad = __syncthreads_or(bad);  // `together` is the same for the whole CTA
-#pragma unroll
-      for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, sh_max[w]);
-      __syncthreads();
-    } else {
-      for (int p = me; p < n * LPT; p += 32)
-        amax = fmaxf(amax, amax8(*reinterpret_cast<const uint4*>(src + (r + p / LPT) * tok + (p % LPT) * 8), bad));
-      amax = warp_max(amax);
-      bad = __any_sync(0xffffffffu, bad);
-    }
-    const int need = need_exponent(amax);
-    const float now = fmaxf(exp2_int(need), old);
-    const float inv = 1.f / now;  // exact: a power of two
-    if (old > 0.f && now > old) {
-      uint2* older = reinterpret_cast<uint2*>(cache + base);
-      for (int p = me; p < off * LPT; p += step) older[p] = rescale8(older[p], old * inv);
-    }
-    uint2* dst = reinterpret_cast<uint2*>(cache + base) + (long)off * LPT;
-    if (together) {
-#pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
-        const int p = me + i * kAppendThreads;
-        if (p < n * LPT) dst[p] = codes8(held[i], inv);
+      for (int b = 0; b < PAGE; b += 32) {
+        const bool in = b + lane < most && slots[r + b + lane] == s0 + b + lane;
+        const uint32_t m = __ballot_sync(0xffffffffu, in);
+        if (on) n += m == 0xffffffffu ? 32 : __ffs(~m) - 1;
+        on = on && m == 0xffffffffu;
       }
-    } else {
-      for (int p = me; p < n * LPT; p += 32)
-        dst[p] = codes8(*reinterpret_cast<const uint4*>(src + (r + p / LPT) * tok + (p % LPT) * 8), inv);
+      const int step = together ? kAppendThreads : 32, me = together ? tid : lane;
+      uint32_t big = 0;
+      auto largest = [&](auto of) {  // over the run's threads
+        uint32_t v = 0;
+        if (together) {
+#pragma unroll
+          for (int i = 0; i < kHeld; ++i)
+            if (tid + i * kAppendThreads < n * LPT) v = of(held[i], v);
+        } else {
+          for (int p = lane; p < n * LPT; p += 32) v = of(piece(p), v);
+        }
+        v = __reduce_max_sync(0xffffffffu, max(v & 0xffffu, v >> 16));
+        if (together) {  // the same for the whole CTA
+          if (lane == 0) sh_max[warp] = v;
+          __syncthreads();
+#pragma unroll
+          for (int w = 0; w < kAppendWarps; ++w) v = max(v, sh_max[w]);
+          __syncthreads();
+        }
+        return v;
+      };
+      big = largest([](const uint4& u, uint32_t v) { return amax8(u, v); });
+      const bool bad = big >= 0x7f80u;  // something is not finite
+      if (bad) big = largest([](const uint4& u, uint32_t v) { return finite8(u, v); });
+      const float now = fmaxf(exp2_int(need_exponent(__uint_as_float(big << 16))), old);
+      const float inv = 1.f / now;  // exact: a power of two
+      if (old > 0.f && now > old) {
+        uint2* older = reinterpret_cast<uint2*>(cache + base);
+        for (int p = me; p < off * LPT; p += step) older[p] = rescale8(older[p], old * inv);
+      }
+      uint2* dst = reinterpret_cast<uint2*>(cache + base) + (long)off * LPT;
+      if (together) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+          const int p = tid + i * kAppendThreads;
+          if (p < n * LPT) dst[p] = bad ? codes8<true>(held[i], inv) : codes8<false>(held[i], inv);
+        }
+      } else {
+        for (int p = lane; p < n * LPT; p += 32) dst[p] = codes8<true>(piece(p), inv);
+        __syncwarp();
+      }
+      // every thread has read `was`: the maxima met in between
+      if (me == 0) *sp = is_v && (bad || was < 0.f) ? -now : now;
     }
-    // every thread has read `was` before the barrier above
-    if (me == 0) *sp = is_v && (bad || was < 0.f) ? -now : now;
   }
+}
+
+template <int HD>
+int launch_append(const Kv8Cache& c, const void* k, const void* v, long k_tok, long v_tok, const int* slots, int rows,
+                  int window, cudaStream_t st) {
+  const dim3 grid((rows + window - 1) / window, c.hkv, 2);
+  auto kernel = c.page == 32 ? append_kernel<HD, 32> : c.page == 64 ? append_kernel<HD, 64> : append_kernel<HD, 128>;
+  count_launch();
+  return launch_early(kernel, grid, kAppendThreads, 0, st, 1, c, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, k_tok,
+                      v_tok, slots, rows, window) == cudaSuccess
+             ? 0
+             : kErrBadArgsHost;
 }
 
 }  // namespace
@@ -194,19 +222,12 @@ __global__ void __launch_bounds__(kAppendThreads)
 int launch_kv8_append(const Kv8Cache& c, const void* k, const void* v, long k_tok, long v_tok, const int* slots,
                       int rows, cudaStream_t st) {
   if (rows < 1) return 0;
-  if (c.page < 1 || c.page > kMaxPage) return kErrBadArgsHost;
+  if (c.page != 32 && c.page != 64 && c.page != 128) return kErrBadArgsHost;
+  // Few rows are a decode step's: a window of 8 gives each run a warp of its own.
   const int window = rows <= 2048 ? 8 : 32;
-  dim3 grid((rows + window - 1) / window, c.hkv, 2);
-  count_launch();
-  if (c.hd == 64)
-    append_kernel<64><<<grid, kAppendThreads, 0, st>>>(c, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, k_tok, v_tok,
-                                                       slots, rows, window);
-  else if (c.hd == 128)
-    append_kernel<128><<<grid, kAppendThreads, 0, st>>>(c, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, k_tok,
-                                                        v_tok, slots, rows, window);
-  else
-    return kErrBadArgsHost;
-  return cudaGetLastError() == cudaSuccess ? 0 : kErrBadArgsHost;
+  if (c.hd == 64) return launch_append<64>(c, k, v, k_tok, v_tok, slots, rows, window, st);
+  if (c.hd == 128) return launch_append<128>(c, k, v, k_tok, v_tok, slots, rows, window, st);
+  return kErrBadArgsHost;
 }
 
 }  // namespace mxk

@@ -34,6 +34,7 @@
 #include <atomic>
 
 #include "kernels.h"
+#include "pdl.cuh"
 
 namespace mxk {
 namespace {
@@ -294,8 +295,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ)) attention_k
   const int g = lane >> 2, t = lane & 3;
   const int rep = args.rep.d, cap = a.width << args.page_shift;
   const Work w = work_of(a.work, a.grid, kRows, HD);
-  // the join's CTAs may take their places; they wait for this grid's end before they read
-  if (!CLUSTER) asm volatile("griddepcontrol.launch_dependents;");
+
+  if (tid == 0) sh_any_nan = 0;
+  for (int x = tid; x < kRows * HD / 4; x += kThreads) reinterpret_cast<int*>(sh_nan)[x] = 0;
+  wait_for_previous();
+  if (!CLUSTER) let_next_start();
 
   // Steps (with CLUSTER segments) before each request, each thread's requests in a row. Ascending
   // starts keep the sum below the host's bound; with any other nothing is computed.
@@ -309,8 +313,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ)) attention_k
   int mine = 0, bad = 0;
   for (int i = 0; i < per; ++i)
     if (tid * per + i < a.R) mine += weight(tid * per + i, bad);
-  if (tid == 0) sh_any_nan = 0;
-  for (int x = tid; x < kRows * HD / 4; x += kThreads) reinterpret_cast<int*>(sh_nan)[x] = 0;
   int x = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -757,7 +759,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
   const int row = blockIdx.x / a.H, h = blockIdx.x % a.H;
   const Work w = work_of(a.work, a.grid, a.tile, HD);
   const int rep = args.rep.d;
-  // the caller's own inputs, complete before the attention kernel began
+  wait_for_previous();
   int r = row;
   if (a.starts != nullptr) {
     if (row >= a.starts[a.R]) return;
@@ -765,12 +767,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
   }
   int row0;
   if (row - (a.starts ? a.starts[r] : r) >= new_rows(a, r, row0)) return;
-  const int steps = steps_of(a.width << args.page_shift, a.lens[r]);
-  if (steps == 1) return;  // one step has one CTA
-  const int kh = args.rep.by(h), x = (row - row0) * rep + h - kh * rep, tile = x / a.tile, y = x % a.tile;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int total = w.prefix[a.R], start = w.prefix[r];
-  if (total == 0) return;
+  const int steps = steps_of(a.width << args.page_shift, a.lens[r]);
+  if (steps == 1 || total == 0) return;  // one step has one CTA
+  const int kh = args.rep.by(h), x = (row - row0) * rep + h - kh * rep, tile = x / a.tile, y = x % a.tile;
   const Share share(total, used_ctas(a, total));
   const int s0 = start + (tile * c.hkv + kh) * steps;
   const int c0 = share.cta(s0), c1 = share.cta(s0 + steps - 1);
@@ -827,30 +827,15 @@ int launch(const Args& args, cudaStream_t st) {
       return kErrBadArgsHost;
     raised[dev].store(true);
   }
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3((unsigned)a.grid);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kRing + (a.R + 1) * 4;
-  cfg.stream = st;
-  cfg.attrs = attr;
   count_launch();
-  if (CLUSTER) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = a.cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_kernel<HD, NQ, CLUSTER>, args) == cudaSuccess ? 0 : kErrBadArgsHost;
-  }
-  if (cudaLaunchKernelEx(&cfg, attention_kernel<HD, NQ, CLUSTER>, args) != cudaSuccess) return kErrBadArgsHost;
-  cfg.gridDim = dim3((unsigned)(a.rows * a.H));
-  cfg.blockDim = dim3(32 * kJoinWarps);
-  cfg.dynamicSmemBytes = 0;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.numAttrs = 1;
+  if (launch_early(attention_kernel<HD, NQ, CLUSTER>, dim3((unsigned)a.grid), kThreads, kRing + (a.R + 1) * 4, st,
+                   CLUSTER ? a.cluster : 1, args) != cudaSuccess)
+    return kErrBadArgsHost;
+  if (CLUSTER) return 0;
   count_launch();
-  return cudaLaunchKernelEx(&cfg, join_kernel<HD>, args) == cudaSuccess ? 0 : kErrBadArgsHost;
+  return launch_early(join_kernel<HD>, dim3((unsigned)(a.rows * a.H)), 32 * kJoinWarps, 0, st, 1, args) == cudaSuccess
+             ? 0
+             : kErrBadArgsHost;
 }
 
 }  // namespace

@@ -25,6 +25,7 @@
 #include <atomic>
 
 #include "kernels.h"
+#include "pdl.cuh"
 
 namespace mxk {
 namespace {
@@ -100,7 +101,7 @@ template <bool GLU>
 __global__ void __launch_bounds__(256) slices_kernel(const __grid_constant__ W4Args a) {
   const int cols = GLU ? a.N / 2 : a.N;
   const long wide = (a.N + 15) / 16 * 16L, i = blockIdx.x * 256L + threadIdx.x;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_previous();
   if (i >= (long)a.T * cols) return;
   const int tok = (int)(i / cols), n = (int)(i % cols);
   const float* p = a.parts + tok * wide + (GLU ? n / 8 * 16 + n % 8 : n);
@@ -240,8 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
   if (pos < end) set_rows();
   for (int i = tid; i < 2 * kWarps; i += kThreads) part_tile[i] = -1;
   // launched early: the kernel before may still be writing x (or the weights)
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (a.slices > 1) asm volatile("griddepcontrol.launch_dependents;");
+  wait_for_previous();
+  if (a.slices > 1) let_next_start();
   // x before the weights, which would keep the memory busy for longer than it waits.
   // Blocks that the last unit lacks meet zeros (their codes are what the ring held).
   for (int c = tid; c < units * BU * 16; c += kThreads) {
@@ -452,25 +453,15 @@ int run(const W4Args& a, int ctas, cudaStream_t st) {
       return kErrBadArgsHost;
     raised[dev].store(true);
   }
-  // Both kernels start while the one before ends; they wait for its end before they read or write.
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(ctas, a.slices);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   count_launch();
-  if (cudaLaunchKernelEx(&cfg, stream_kernel<NT, GW, GLU>, a) != cudaSuccess) return kErrBadArgsHost;
+  if (launch_early(stream_kernel<NT, GW, GLU>, dim3(ctas, a.slices), kThreads, smem, st, 1, a) != cudaSuccess)
+    return kErrBadArgsHost;
   if (a.slices == 1) return 0;
-  cfg.gridDim = dim3((unsigned)(((long)a.T * (GLU ? a.N / 2 : a.N) + 255) / 256));
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = 0;
   count_launch();
-  return cudaLaunchKernelEx(&cfg, slices_kernel<GLU>, a) == cudaSuccess ? 0 : kErrBadArgsHost;
+  const long outputs = (long)a.T * (GLU ? a.N / 2 : a.N);
+  return launch_early(slices_kernel<GLU>, dim3((unsigned)((outputs + 255) / 256)), 256, 0, st, 1, a) == cudaSuccess
+             ? 0
+             : kErrBadArgsHost;
 }
 template <int NT>
 int run_group(const W4Args& a, int group, bool glu, int ctas, cudaStream_t st) {
