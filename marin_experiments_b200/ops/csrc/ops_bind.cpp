@@ -574,19 +574,17 @@ std::vector<Tensor> block_tables_extend(const Tensor& tables, const Tensor& lens
   need(free_pages.numel() * page < (1LL << 31) && tables.size(1) * page < (1LL << 31),
        "a pool or a table of 2^31 tokens or more");
   c10::cuda::CUDAGuard g(tables.device());
-  // one buffer: lens [R], starts [R + 1], free_count, status, slots, requests, positions [rows]
+  const at::AutoDispatchBelowADInplaceOrView plain;  // views without autograd's records
+  // one buffer: lens [R], free_count, starts [R + 1], slots, requests, positions [rows], status
   Tensor buf = at::empty({2 * R + 3 + 3 * rows}, tables.options());
   int* b = buf.data_ptr<int>();
-  int* sl = b + 2 * R + 3;
+  int* sl = b + 2 * R + 2;
   ok(mxk::launch_block_tables_extend(tables.data_ptr<int>(), (int)tables.size(1), lens.data_ptr<int>(),
                                      grow.data_ptr<int>(), (int)R, free_pages.data_ptr<int>(),
                                      (int)free_pages.numel(), free_count.data_ptr<int>(), (int)page, (int)rows, b,
-                                     b + 2 * R + 1, b + R, sl, sl + rows, sl + 2 * rows, b + 2 * R + 2, stream()),
+                                     b + R, b + R + 1, sl, sl + rows, sl + 2 * rows, sl + 3 * rows, stream()),
      "block_tables_extend");
-  auto part = [&](int64_t at, int64_t n) { return buf.narrow(0, at, n); };
-  const int64_t s = 2 * R + 3;
-  return {part(0, R), part(2 * R + 1, 1), part(R, R + 1), part(s, rows), part(s + rows, rows),
-          part(s + 2 * rows, rows), part(2 * R + 2, 1)};
+  return buf.split_with_sizes({R, 1, R + 1, rows, rows, rows, 1});
 }
 
 Tensor block_tables_release(const Tensor& tables, const Tensor& lens, const Tensor& done, const Tensor& free_pages,
@@ -602,6 +600,7 @@ Tensor block_tables_release(const Tensor& tables, const Tensor& lens, const Tens
   need(R >= 1 && R <= mxk::kTablesMaxRequests, "between 1 and 4096 requests");
   need(page >= 1, "page must be positive");
   c10::cuda::CUDAGuard g(tables.device());
+  const at::AutoDispatchBelowADInplaceOrView plain;
   Tensor status = at::empty({1}, tables.options());
   ok(mxk::launch_block_tables_release(tables.data_ptr<int>(), (int)tables.size(1), lens.data_ptr<int>(),
                                       (const uint8_t*)done.data_ptr(), (int)R, free_pages.data_ptr<int>(),
@@ -677,6 +676,7 @@ Tensor kv8_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const 
   }
   need(T < (1LL << 31) - 64 && R >= 1 && R <= mxk::kTablesMaxRequests && H <= 65535, "between 1 and 4096 requests");
   c10::cuda::CUDAGuard g(kc.device());
+  const at::AutoDispatchBelowADInplaceOrView plain;
   Tensor o;
   if (out.has_value()) {
     o = *out;
@@ -742,6 +742,7 @@ Tensor linear_w4(const Tensor& x, const Tensor& codes, const Tensor& scales, con
     need(residual->size(0) == x.size(0), "one residual row for each row of x");
   }
   c10::cuda::CUDAGuard g(codes.device());
+  const at::AutoDispatchBelowADInplaceOrView plain;
   Tensor out = at::empty({x.size(0), glu ? N / 2 : N}, x.options()), work;
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   const long floats = mxk::linear_w4_work((int)x.size(0), (int)N, (int)K, sms);
