@@ -166,7 +166,7 @@ def build_app(engine, model_name: str = "qwen3"):
     return app
 
 
-def tiny_engine(device="cpu"):
+def tiny_engine(device="cpu", **options):
     """A small random-init Qwen3 with the byte tokenizer (tests and smoke runs)."""
     from ..data.tokenize import ByteTokenizer
     from ..models.qwen3 import Qwen3Config, Qwen3Model
@@ -175,7 +175,7 @@ def tiny_engine(device="cpu"):
     cfg = Qwen3Config(vocab_size=512, hidden_dim=128, intermediate_dim=256, num_layers=2, num_heads=2, num_kv_heads=1,
                       head_dim=64, rope_theta=10000.0, max_seq_len=256)
     model = Qwen3Model(cfg).init_weights(0).to(device)
-    return Engine(model, ByteTokenizer(), device=device, max_batch=4, max_len=256)
+    return Engine(model, ByteTokenizer(), device=device, max_batch=4, max_len=256, **options)
 
 
 def main(argv=None):
@@ -189,17 +189,20 @@ def main(argv=None):
     ap.add_argument("--host", default="127.0.0.1")
     ap.add_argument("--port", type=int, default=8000)
     ap.add_argument("--max-batch", type=int, default=8)
+    ap.add_argument("--kv-cache", choices=("bf16", "fp8"), default="bf16", help="fp8: paged 8-bit KV cache (GPU)")
+    ap.add_argument("--weights", choices=("bf16", "int4"), default="bf16", help="int4: 4-bit weights (GPU)")
     args = ap.parse_args(argv)
     dev = "cuda" if torch.cuda.is_available() else "cpu"
     if args.random_tiny or not args.model_dir:
-        engine, name = tiny_engine(dev), "random-tiny"
+        engine, name = tiny_engine(dev, kv_cache=args.kv_cache, weights=args.weights), "random-tiny"
     else:
         from ..data.tokenize import load_tokenizer
         from ..models.qwen3 import load_hf
         from .engine import Engine
 
         model = load_hf(args.model_dir, device=dev)
-        engine = Engine(model, load_tokenizer(args.tokenizer or args.model_dir), device=dev, max_batch=args.max_batch)
+        engine = Engine(model, load_tokenizer(args.tokenizer or args.model_dir), device=dev, max_batch=args.max_batch,
+                        kv_cache=args.kv_cache, weights=args.weights)
         name = args.model_dir
     uvicorn.run(build_app(engine, name), host=args.host, port=args.port)
 

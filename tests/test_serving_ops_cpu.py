@@ -178,3 +178,12 @@ def test_refusals():
     c = O.make_cache([4], hkv=1, hd=64, page=32)
     with pytest.raises(RuntimeError):
         attend(torch.randn(1, 1, 64).requires_grad_(), c)
+
+
+def test_engine_refuses_the_quantised_options_without_a_gpu():
+    from marin_experiments_b200.serving.server import tiny_engine
+
+    for kw in ({"kv_cache": "fp8"}, {"weights": "int4"}, {"kv_cache": "int8"}, {"weights": "fp4"}):
+        with pytest.raises(ValueError):
+            tiny_engine("cpu", **kw)
+    assert tiny_engine("cpu", kv_cache="bf16", weights="bf16").ready
