@@ -102,10 +102,10 @@ __device__ __forceinline__ uint2 rescale8(uint2 u, float ratio) {
 constexpr int kAppendThreads = 256;
 constexpr int kAppendWarps = kAppendThreads / 32;
 
-// Pages of 128 hold 8 pieces a thread: held to 3 CTAs an SM (16000 rows 24.3 -> 19.1 us); others gain
-// nothing from fewer registers.
+// Pages of 128 hold 8 pieces a thread: held to 3 CTAs an SM (16000 rows 24.3 -> 19.1 us),
+// the others to 4 (7000 rows in pages of 64: 15 us; 23 at one, where registers are not held back).
 template <int HD, int PAGE>
-__global__ void __launch_bounds__(kAppendThreads, PAGE == 128 ? 3 : 1)
+__global__ void __launch_bounds__(kAppendThreads, PAGE == 128 ? 3 : 4)
     append_kernel(const __grid_constant__ Kv8Cache c, const __nv_bfloat16* __restrict__ k_new,
                   const __nv_bfloat16* __restrict__ v_new, long k_tok, long v_tok, const int* __restrict__ slots,
                   int rows, int window) {
