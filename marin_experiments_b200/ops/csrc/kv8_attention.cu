@@ -339,12 +339,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ)) attention_k
   __syncthreads();
   if (!CLUSTER && blockIdx.x == 0)
     for (int r = tid; r <= a.R; r += kThreads) w.prefix[r] = prefix[r];
-  if (a.zero_tail) {  // rows behind the last request
-    const int last = max(0, min(a.rows, a.starts[a.R]));
-    uint4* o = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (long)last * a.H * HD);
-    const long n = (long)(a.rows - last) * a.H * HD / 8;
+  if (a.zero_tail) {  // rows of no request: before the first, behind the last, all if starts do not ascend
+    const int last = bad ? 0 : max(0, min(a.rows, a.starts[a.R]));
+    const int lead = bad ? 0 : max(0, min(last, a.starts[0]));
+    constexpr int kPieces = HD / 8;
+    const long per = (long)a.H * kPieces, n = (a.rows - last + lead) * per;
+    uint4* o = reinterpret_cast<uint4*>(a.out);
     for (long i = blockIdx.x * (long)kThreads + tid; i < n; i += (long)gridDim.x * kThreads)
-      o[i] = make_uint4(0, 0, 0, 0);
+      o[i < lead * per ? i : i - lead * per + last * per] = make_uint4(0, 0, 0, 0);
   }
 
   const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(smem), ring = ring0 + warp * kStages * kStageBytes;
@@ -842,7 +844,7 @@ int launch(const Args& args, cudaStream_t st) {
 
 bool kv8_attention_plan(Kv8Attention& a, int hkv, int page, int hd, int sms) {
   if (a.R < 1 || a.R > kMaxRequests || a.rows < 0 || hkv < 1 || a.H % hkv) return false;
-  if ((long)a.width * page > 0x7fffffffL || (long)a.rows * a.H > 0x7fffffffL) return false;
+  if ((long)a.width * page > 1 << 30 || (long)a.rows * a.H > 1 << 30) return false;
   // Rows of a tile: what a request's rows of one kv head need on average (8 in decode up to 8 query
   // heads a group), 16 at most at hd 128 and 32 at hd 64, where the registers end.
   const long n = ((long)a.rows + a.R - 1) / a.R * (a.H / hkv);

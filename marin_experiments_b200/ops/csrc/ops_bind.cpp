@@ -570,9 +570,9 @@ std::vector<Tensor> block_tables_extend(const Tensor& tables, const Tensor& lens
   const int64_t R = tables.size(0);
   need(lens.size(0) == R && grow.size(0) == R, "one length and one new length for each row of the tables");
   need(R >= 1 && R <= mxk::kTablesMaxRequests, "between 1 and 4096 requests");
-  need(page >= 1 && rows >= 0 && rows < (1LL << 31) - 1, "page must be positive and rows not negative");
-  need(free_pages.numel() * page < (1LL << 31) && tables.size(1) * page < (1LL << 31),
-       "a pool or a table of 2^31 tokens or more");
+  need(page >= 1 && rows >= 0 && rows <= 1LL << 30, "page must be positive and rows between 0 and 2^30");
+  need(page <= 1LL << 30 && free_pages.numel() * page <= 1LL << 30 && tables.size(1) * page <= 1LL << 30,
+       "a pool or a table of more than 2^30 tokens");
   c10::cuda::CUDAGuard g(tables.device());
   const at::AutoDispatchBelowADInplaceOrView plain;  // views without autograd's records
   // one buffer: lens [R], free_count, starts [R + 1], slots, requests, positions [rows], status
@@ -598,7 +598,8 @@ Tensor block_tables_release(const Tensor& tables, const Tensor& lens, const Tens
   const int64_t R = tables.size(0);
   need(lens.size(0) == R && done.size(0) == R, "one length and one mark for each row of the tables");
   need(R >= 1 && R <= mxk::kTablesMaxRequests, "between 1 and 4096 requests");
-  need(page >= 1, "page must be positive");
+  need(page >= 1 && page <= 1LL << 30 && free_pages.numel() <= 1LL << 30 && tables.size(1) * page <= 1LL << 30,
+       "page must be positive, and a table at most 2^30 tokens");
   c10::cuda::CUDAGuard g(tables.device());
   const at::AutoDispatchBelowADInplaceOrView plain;
   Tensor status = at::empty({1}, tables.options());
@@ -650,7 +651,7 @@ void kv8_append(const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor
   cuda_i32(slots, "slots");
   same_device(kc, {&k, &v, &slots});
   need(k.size(0) == v.size(0) && slots.dim() == 1 && slots.size(0) == k.size(0), "one slot for each row of k and v");
-  need(k.size(0) < (1LL << 31) - 64, "too many rows");
+  need(k.size(0) <= 1LL << 30, "more than 2^30 rows");
   c10::cuda::CUDAGuard g(kc.device());
   ok(mxk::launch_kv8_append(c, k.data_ptr(), v.data_ptr(), kt, vt, slots.data_ptr<int>(), (int)k.size(0), stream()),
      "kv8_append");
@@ -674,7 +675,7 @@ Tensor kv8_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const 
   } else {
     need(T == R, "without starts there is one row for each request");
   }
-  need(T < (1LL << 31) - 64 && R >= 1 && R <= mxk::kTablesMaxRequests && H <= 65535, "between 1 and 4096 requests");
+  need(T <= 1LL << 30 && R >= 1 && R <= mxk::kTablesMaxRequests && H <= 65535, "between 1 and 4096 requests");
   c10::cuda::CUDAGuard g(kc.device());
   const at::AutoDispatchBelowADInplaceOrView plain;
   Tensor o;
@@ -713,7 +714,7 @@ int w4_group(const Tensor& codes, const Tensor& scales) {
   same_device(codes, {&scales});
   aligned16(codes, "codes");
   const int64_t N = codes.size(0), K = codes.size(1) * 8;
-  need(N >= 1 && K >= 128 && K % 128 == 0 && N < (1LL << 31) - 64 && K < (1LL << 30), "K must be a multiple of 128");
+  need(N >= 1 && K >= 128 && K % 128 == 0 && N <= 1LL << 30 && K <= 1LL << 24, "K must be a multiple of 128 up to 2^24, and N at most 2^30");
   need(scales.dim() == 2 && scales.size(0) == N && scales.size(1) >= 1 && K % scales.size(1) == 0,
        "scales must be [N, K / group]");
   const int64_t group = K / scales.size(1);

@@ -420,6 +420,8 @@ def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, tables, lens, starts=No
     scale = hd ** -0.5 if scale is None else scale
     o = torch.zeros_like(q) if out is None else out
     st = list(range(rows + 1)) if starts is None else starts.tolist()
+    if st != sorted(st) or st[0] < 0 or st[-1] > rows:
+        return o
     for r, n in enumerate(lens.tolist()):
         a, b = st[r], st[r + 1]
         for i in range(a, b):

@@ -6,6 +6,7 @@ import torch
 
 from marin_experiments_b200.ops import api
 from marin_experiments_b200.ops import reference as R
+from marin_experiments_b200.ops.quant import unpack_w4
 
 import serving_ops_oracle as O
 
@@ -308,6 +309,46 @@ def test_attention_starts_that_do_not_ascend():
     attend(q, c, starts=torch.tensor([0, 8, 2, 8], dtype=torch.int32, device="cuda"), out=out)
     attend(q, c, starts=torch.tensor([-4, 8, 900, 901], dtype=torch.int32, device="cuda"), out=out)
     assert bool((out == 3).all())
+    assert not bool(attend(q, c, starts=torch.tensor([0, 8, 2, 8], dtype=torch.int32, device="cuda")).any())
+    # rows before the first request belong to none either
+    st = torch.tensor([2, 3, 3, 5], dtype=torch.int32, device="cuda")
+    got = attend(q, c, starts=st)
+    assert not bool(got[:2].any()) and not bool(got[5:].any()) and bool(got[2:5].any(-1).all())
+
+
+def test_attention_of_a_long_prompt():
+    """Hundreds of new rows: many row tiles of one request, each with its own last position."""
+    c = O.make_cache([700, 300], hkv=2, hd=64, page=64, seed=5)
+    starts = [0, 411, 711]
+    q = torch.randn(711, 6, 64, generator=torch.Generator().manual_seed(1)).to(BF16)
+    want, size = O.attention64(q, c, starts)
+    got = attend(q.cuda(), cuda(c), starts=torch.tensor(starts, dtype=torch.int32, device="cuda"))
+    O.close(got, want, O.attention_bound(want, size))
+
+
+def test_cache_beyond_32_bit_offsets():
+    """Append to, and attention over, pages more than 2^32 bytes into the cache."""
+    pages, hkv, page, hd = 70_000, 8, 64, 128
+    k, v = (torch.empty(pages, hkv, page, hd, dtype=torch.uint8, device="cuda").view(O.E4M3) for _ in range(2))
+    ks, vs = (torch.zeros(pages, hkv, device="cuda") for _ in range(2))
+    table = torch.tensor([[69_999, 3, 66_000]], dtype=torch.int32, device="cuda")
+    n = 150
+    pos = torch.arange(n, device="cuda")
+    slots = (table[0, pos // page] * page + pos % page).int()
+    g = torch.Generator().manual_seed(0)
+    kn, vn = (torch.randn(n, hkv, hd, generator=g).to(BF16) for _ in range(2))
+    api.kv8_append(kn.cuda(), vn.cuda(), k, v, ks, vs, slots)
+    small = {"k": torch.zeros(3, hkv, page, hd).to(O.E4M3), "ks": torch.zeros(3, hkv)}
+    small |= {"v": small["k"].clone(), "vs": small["ks"].clone(), "tables": torch.tensor([[0, 1, 2]], dtype=torch.int32),
+              "lens": torch.tensor([n], dtype=torch.int32)}
+    R.kv8_append(kn, vn, small["k"], small["v"], small["ks"], small["vs"], torch.arange(n).int())
+    at = table[0].long()
+    same_codes(k.view(torch.uint8)[at][2, :, : n - 2 * page], small["k"][2, :, : n - 2 * page])
+    assert torch.equal(vs[at].cpu(), small["vs"])
+    q = torch.randn(1, 16, hd, generator=g).to(BF16)
+    got = api.kv8_attention(q.cuda(), k, v, ks, vs, table, torch.tensor([n], dtype=torch.int32, device="cuda"))
+    want, size = O.attention64(q, small)
+    O.close(got, want, O.attention_bound(want, size))
 
 
 # -------------------------------------------------------------------------------- 4-bit weights
@@ -371,6 +412,20 @@ def test_linear_w4_many_rows(n, glu):
     y2 = y + res.double()
     O.close(api.linear_w4(x.cuda(), packed.cuda(), scales.cuda(), residual=res.cuda()), y2,
             2.0**-8 * (y2.abs() + y.abs()) * 1.01 + e * 1.01)
+
+
+def test_linear_w4_beyond_32_bit_offsets():
+    """A matrix of more than 2^32 bytes of codes; its last rows."""
+    n, k = 550_000, 16384
+    words = torch.randint(-(2**31), 2**31, (1000, k // 8), device="cuda").int()
+    codes = torch.empty(n, k // 8, dtype=torch.int32, device="cuda")
+    codes[-1000:] = words
+    codes[:-1000].zero_()
+    scales = torch.full((n, k // 128), 0.01, dtype=BF16, device="cuda")
+    x = torch.randn(2, k, device="cuda").to(BF16)
+    got = api.linear_w4(x, codes, scales)
+    y, size = O.w4_64(x.cpu(), unpack_w4(words.cpu()), scales[-1000:].cpu())
+    O.close(got[:, -1000:], y, O.w4_bound(y, size, k))
 
 
 def test_linear_w4_nan_scale_shows():
@@ -486,7 +541,8 @@ def test_refusals():
     v = torch.zeros(2, dtype=torch.int32, device="cuda")
     one = torch.zeros(1, dtype=torch.int32, device="cuda")
     bad += [lambda: api.block_tables_extend(t, v[:1], v, v, one, 32, 4), lambda: api.block_tables_extend(t, v, v, v, v, 32, 4),
-            lambda: api.block_tables_extend(t, v, v, v, one, 0, 4), lambda: api.block_tables_extend(t, v, v, v, one, 32, -1),
+            lambda: api.block_tables_extend(t, v, v, v, one, 0, 4), lambda: api.block_tables_extend(t, v, v, v, one, 32, 2**31 - 2),
+            lambda: api.block_tables_extend(t, v, v, v, one, 2**30, 4), lambda: api.block_tables_extend(t, v, v, v, one, 32, -1),
             lambda: api.block_tables_release(t, v, v, v, one, 32)]
     for f in bad:
         with pytest.raises((RuntimeError, ValueError)):
