@@ -44,7 +44,6 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kChunk = 32;           // keys a warp takes at once: always inside one page
 constexpr int kStep = kChunk * kWarps;
 constexpr int kMaxRequests = 4096;
-constexpr int kStages = 2;
 constexpr int kJoinWarps = 8;
 // Long calls make up to kRounds CTAs for each that runs at once, of kManySteps steps or more: SMs are
 // not equally fast, and the hardware gives the next CTA to the one that is free (48 requests of up to
@@ -53,10 +52,13 @@ constexpr long kRounds = 8;
 constexpr int kManySteps = 16;
 constexpr int kClusterSteps = 16;    // most steps a CTA of a cluster takes
 
-// CTAs an SM: what its registers hold without spilling (255 at two, 168 at three, 128 at four), and
-// at most what 228 KB of shared memory hold of rings (64 KB at hd 128, 32 KB at hd 64).
-__host__ __device__ constexpr int ctas_per_sm(int hd, int tile) {
-  return hd == 128 ? (tile == 8 ? 3 : 2) : (tile == 8 ? 4 : 3);
+// Chunks of a warp on their way, and CTAs an SM: what its registers hold without spilling (255 at
+// two, 168 at three, 128 at four), and 228 KB of shared memory hold of rings (a stage is 32 KB of a
+// CTA at hd 128). A cluster's CTAs have few chunks each, whose latency counts: a stage more for a CTA
+// less.
+__host__ __device__ constexpr int stages_of(int hd, bool cluster) { return hd == 128 ? (cluster ? 3 : 2) : (cluster ? 4 : 3); }
+__host__ __device__ constexpr int ctas_per_sm(int hd, int tile, bool cluster) {
+  return hd == 128 ? (tile == 8 && !cluster ? 3 : 2) : (tile == 8 && !cluster ? 4 : 3);
 }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
@@ -275,8 +277,8 @@ __device__ __noinline__ void take_out_nan(uint8_t* values, uint8_t* marks, int l
 
 // NQ: tiles of 8 rows that a segment's rows form. CLUSTER: one segment for each cluster.
 template <int HD, int NQ, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ)) attention_kernel(const __grid_constant__ Args args) {
-  constexpr int kRows = 8 * NQ;
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) attention_kernel(const __grid_constant__ Args args) {
+  constexpr int kRows = 8 * NQ, kStages = stages_of(HD, CLUSTER);
   constexpr int KB = HD / 64;              // 16-byte pieces of a key a lane reads
   constexpr int MT = HD / 16;              // tiles of 16 dims of the output
   constexpr int E = HD / 32;               // dims of an output row a lane joins
@@ -815,7 +817,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 
 template <int HD, int NQ, bool CLUSTER>
 int launch(const Args& args, cudaStream_t st) {
-  constexpr int kRing = kWarps * kStages * 2 * kChunk * HD;
+  constexpr int kRing = kWarps * stages_of(HD, CLUSTER) * 2 * kChunk * HD;
   static_assert(kWarps * 8 * NQ * HD * 4 <= kRing, "the join fits the ring");
   static_assert(!CLUSTER || (kWarps + 1) * 8 * NQ * HD * 4 + 64 * NQ <= kRing, "so does a cluster's part");
   const Kv8Attention& a = args.a;
@@ -853,12 +855,12 @@ bool kv8_attention_plan(Kv8Attention& a, int hkv, int page, int hd, int sms) {
   const long steps = std::max(1L, ((long)a.width * page + kStep - 1) / kStep);
   const long segs = a.starts == nullptr ? (long)a.R * hkv * ((a.H / hkv + a.tile - 1) / a.tile) : tiles * hkv;
   if ((double)tiles * hkv * steps > 2.0e9) return false;
-  const long ctas = (long)sms * ctas_per_sm(hd, a.tile);
+  const long ctas = (long)sms * ctas_per_sm(hd, a.tile, false), at_once = (long)sms * ctas_per_sm(hd, a.tile, true);
   a.cluster = 0;
   int size = 8;
-  while (size > 1 && segs * size > ctas) size /= 2;
+  while (size > 1 && segs * size > at_once) size /= 2;
   while (size > 1 && size / 2 >= steps) size /= 2;
-  if (a.tile <= 16 && segs * size <= ctas && steps <= (long)kClusterSteps * size) {
+  if (a.tile <= 16 && segs * size <= at_once && steps <= (long)kClusterSteps * size) {
     a.cluster = size;
     a.grid = (int)(segs * size);
   } else {
