@@ -61,7 +61,10 @@ __host__ __device__ constexpr int ctas_per_sm(int hd, int tile, bool cluster) {
   return hd == 128 ? (tile == 8 && !cluster ? 3 : 2) : (tile == 8 && !cluster ? 4 : 3);
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src));
+}
+__device__ __forceinline__ void cp16_if(uint32_t dst, const void* src, bool in) {
   const int n = in ? 16 : 0;  // 0: the 16 bytes become zeros, and nothing is read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n));
 }
@@ -352,6 +355,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
   }
 
   const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(smem), ring = ring0 + warp * kStages * kStageBytes;
+  // the lane's place in a stage, of the first of its copies: 4 keys a copy at hd 128, 8 at 64
+  const int col = lane % (HD / 16), row_of = lane / (HD / 16);
+  const int k_place = row_of * HD + (HD == 128 ? col ^ ((row_of & 1) << 2) : col) * 16;
+  const int v_place = row_of * HD + (col ^ (((row_of >> 1) & (HD == 128 ? 3 : 1)) << 1)) * 16;
   int at, end;
   const int parts = CLUSTER ? a.cluster : 1, rank = CLUSTER ? blockIdx.x % parts : 0;
   if (CLUSTER) {
@@ -409,17 +416,18 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
     auto load = [&](int i, bool values) {
       const int key0 = (first + i * kWarps) * kChunk;
       const int pg = __shfl_sync(0xffffffffu, page_id, i & 31);
-      const uint32_t dst = ring + (i % kStages) * kStageBytes + (values ? kChunk * HD : 0);
-      const uint8_t* src = (const uint8_t*)(values ? c.v : c.k) +
+      const uint32_t stage = ring + (i % kStages) * kStageBytes;
+      const uint32_t dst = values ? stage + kChunk * HD + v_place : stage + k_place;
+      const uint8_t* src = (const uint8_t*)(values ? c.v : c.k) + lane * 16 +
                            (((long)max(pg, 0) * c.hkv + kh) * c.page + (key0 & (c.page - 1))) * HD;
+      if (key0 + kChunk <= seen && pg >= 0) {
 #pragma unroll
-      for (int x = 0; x < kLoads; ++x) {
-        const int byte = (x * 32 + lane) * 16, key = byte / HD, col = byte % HD / 16;
-        const bool in = pg >= 0 && key0 + key < seen;  // what lies behind the last key is not read
-        int sw;
-        if (HD == 128) sw = values ? col ^ (((key >> 1) & 3) << 1) : col ^ ((key & 1) << 2);
-        else sw = values ? col ^ (((key >> 1) & 1) << 1) : col;
-        cp16(dst + key * HD + sw * 16, src + byte, in);
+        for (int x = 0; x < kLoads; ++x) cp16((dst + x * 512) ^ (HD == 128 && values && x % 2 ? 64 : 0), src + x * 512);
+      } else {  // what lies behind the last key is not read
+#pragma unroll 1
+        for (int x = 0; x < kLoads; ++x)
+          cp16_if((dst + x * 512) ^ (HD == 128 && values && x % 2 ? 64 : 0), src + x * 512,
+                  pg >= 0 && key0 + (x * 512 + lane * 16) / HD < seen);
       }
       cp_commit();
     };
@@ -559,16 +567,22 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
       float factor[NQ][2];
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
-        float top[2] = {-INFINITY, -INFINITY};
+        const float f0 = qs[n][0] * ks, f1 = qs[n][1] * ks;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            float v = s[h][n][x] * (qs[n][x & 1] * ks);
-            if (diag && key0 + 16 * h + g + 8 * (x >> 1) > pos[n][x & 1]) v = -INFINITY;
-            s[h][n][x] = v;
-            top[x & 1] = fmaxf(top[x & 1], v);
-          }
+          for (int x = 0; x < 4; ++x) s[h][n][x] *= x & 1 ? f1 : f0;
+        if (diag) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (key0 + 16 * h + g + 8 * (x >> 1) > pos[n][x & 1]) s[h][n][x] = -INFINITY;
+        }
+        float top[2];
+#pragma unroll
+        for (int z = 0; z < 2; ++z)
+          top[z] = fmaxf(fmaxf(s[0][n][z], s[0][n][z + 2]), fmaxf(s[1][n][z], s[1][n][z + 2]));
         float sub[2];
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
