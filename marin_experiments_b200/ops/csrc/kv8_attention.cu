@@ -556,10 +556,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
 
       const bool diag = key0 + kChunk > min(len, tile_first + 1);  // some row does not see some key
       float pscale = 1.f, ratio = 1.f;
-      if (fabsf(vs) > 0.f) {  // sums in units of this page's scale (2^-60 of the last at least)
-        const float now = fmaxf(fabsf(vs), unit * 0x1p-60f);
+      const float v_unit = fabsf(vs);
+      if (v_unit != unit && v_unit > 0.f) {  // sums in units of this page's scale (2^-60 of the last at least)
+        const float now = fmaxf(v_unit, unit * 0x1p-60f);
         ratio = unit / now;
-        pscale = fabsf(vs) / now;
+        pscale = v_unit / now;
         unit = now;
       }
       uint32_t pf[NQ][2][2];
@@ -599,10 +600,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
         for (int h = 0; h < 2; ++h) {
           float p[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            p[x] = ex2(s[h][n][x] - sub[x & 1]);
-            l[n][x & 1] += p[x];
-          }
+          for (int x = 0; x < 4; ++x) p[x] = ex2(s[h][n][x] - sub[x & 1]);
+          l[n][0] += p[0] + p[2];
+          l[n][1] += p[1] + p[3];
           if (pscale != 1.f) {
 #pragma unroll
             for (int x = 0; x < 4; ++x) p[x] *= pscale;
