@@ -310,5 +310,6 @@ def linear_w4(x, codes, scales, *, residual=None, glu: bool = False) -> torch.Te
     if not x.is_cuda:
         return R.linear_w4(x, codes, scales, residual, glu)
     if x.shape[0] <= 64:
-        return _cuda().ext().linear_w4(x, codes, scales, residual, glu)
+        fns = _cuda()
+        return fns.ext().linear_w4(x, codes, scales, residual, glu, fns.err_flag(x.device) if x.shape[0] > 16 else None)
     return _cuda().linear_w4_dense(x, codes, scales, residual, glu)

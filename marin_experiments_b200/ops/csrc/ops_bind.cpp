@@ -712,7 +712,7 @@ int w4_group(const Tensor& codes, const Tensor& scales) {
        "codes must be a contiguous CUDA int32 tensor [N, K / 8]");
   cuda_bf16(scales, "scales"); contig(scales, "scales");
   same_device(codes, {&scales});
-  aligned16(codes, "codes");
+  aligned16(codes, "codes"); aligned16(scales, "scales");
   const int64_t N = codes.size(0), K = codes.size(1) * 8;
   need(N >= 1 && K >= 128 && K % 128 == 0 && N <= 1LL << 30 && K <= 1LL << 24, "K must be a multiple of 128 up to 2^24, and N at most 2^30");
   need(scales.dim() == 2 && scales.size(0) == N && scales.size(1) >= 1 && K % scales.size(1) == 0,
@@ -722,7 +722,8 @@ int w4_group(const Tensor& codes, const Tensor& scales) {
   return (int)group;
 }
 
-Tensor linear_w4(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptT& residual, bool glu) {
+Tensor linear_w4(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptT& residual, bool glu,
+                 const OptT& err) {
   const int group = w4_group(codes, scales);
   const int64_t N = codes.size(0), K = codes.size(1) * 8;
   auto rows = [&](const Tensor& t, int64_t cols, int64_t align, const char* n) {
@@ -746,11 +747,16 @@ Tensor linear_w4(const Tensor& x, const Tensor& codes, const Tensor& scales, con
   const at::AutoDispatchBelowADInplaceOrView plain;
   Tensor out = at::empty({x.size(0), glu ? N / 2 : N}, x.options()), work;
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const long floats = mxk::linear_w4_work((int)x.size(0), (int)N, (int)K, sms);
+  if (x.size(0) > 16) {
+    need(err.has_value(), "linear_w4 needs the device's error flag from 17 rows on");
+    cuda_i32(*err, "err");
+    same_device(codes, {&*err});
+  }
+  const long floats = mxk::linear_w4_work((int)x.size(0), (int)N, (int)K, glu, sms);
   if (floats) work = at::empty({floats}, x.options().dtype(at::kFloat));
   ok(mxk::launch_linear_w4(x.data_ptr(), xt, codes.data_ptr(), scales.data_ptr(), ptr<const void>(residual), rt,
                            out.data_ptr(), (int)x.size(0), (int)N, (int)K, group, glu, sms,
-                           floats ? work.data_ptr<float>() : nullptr, stream()),
+                           floats ? work.data_ptr<float>() : nullptr, ptr<int>(err), stream()),
      "linear_w4");
   return out;
 }

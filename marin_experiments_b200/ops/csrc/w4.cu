@@ -26,27 +26,19 @@
 
 #include "kernels.h"
 #include "pdl.cuh"
+#include "w4.cuh"
 
 namespace mxk {
 namespace {
 
 constexpr int kWarps = 16;
+constexpr int kFew = 16;    // rows of x that these kernels take; w4_wide.cu takes more
 constexpr int kStages = 2;  // units of a warp on their way
 // Blocks of 128 values of K in a unit: 256 bytes of a row, or 128 where x needs the shared memory.
 __host__ __device__ constexpr int blocks_of(int nt) { return nt == 1 ? 4 : 2; }
 constexpr int kMaxSmem = 226 * 1024;  // of 227 KB; part_tile is static
 constexpr double kSliceCost = 0.1;  // of one more slice, in units
 constexpr int kThreads = kWarps * 32;
-constexpr int kGlu = 128;  // rows of a gate (or up) block
-
-// (2 j, 2 j + 1) of a word, as bf16 codes. The mask and the exponent go in by one lop3; the compiler
-// makes two of the expression.
-__device__ __forceinline__ uint32_t pair_of(uint32_t w, int j, uint32_t magic, uint32_t bias) {
-  uint32_t u, d;
-  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(u) : "r"(w >> (4 * j)), "r"(magic));
-  asm("sub.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(u), "r"(bias));
-  return d;
-}
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
@@ -63,56 +55,6 @@ __device__ __forceinline__ void mma0(float (&d)[4], uint32_t a0, uint32_t a1, ui
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
-
-struct W4Args {
-  const __nv_bfloat16* x;
-  long x_tok;
-  const uint32_t* codes;
-  const __nv_bfloat16* scales;
-  const __nv_bfloat16* residual;
-  long r_tok;
-  __nv_bfloat16* out;
-  int T, N, K;
-  // blockIdx.y is the slice of K. The CTAs of a slice take `per` tiles each, the first `more` one more;
-  // `whole`: their warps take whole tiles.
-  int slices, per, more, whole;
-  float* parts;  // [slices][T][N rounded up to 16], where there are several slices
-};
-
-// One output of a tile's row r (with GLU a unit, whose gate is y), or this slice's part of it.
-template <bool GLU>
-__device__ __forceinline__ void store(const W4Args& a, int slice, int tile, int r, int tok, float y, float up) {
-  if (a.slices > 1) {
-    float* p = a.parts + ((long)slice * a.T + tok) * ((a.N + 15) / 16 * 16L) + tile * 16 + r;
-    p[0] = y;
-    if (GLU) p[8] = up;
-    return;
-  }
-  const int cols = GLU ? a.N / 2 : a.N, n = tile * (GLU ? 8 : 16) + r;
-  if (n >= cols) return;
-  if (GLU) y = y / (1.f + expf(-y)) * up;
-  if (a.residual) y += __bfloat162float(a.residual[(long)tok * a.r_tok + n]);
-  a.out[(long)tok * cols + n] = __float2bfloat16(y);
-}
-
-// The result from the slices' parts, in their order.
-template <bool GLU>
-__global__ void __launch_bounds__(256) slices_kernel(const __grid_constant__ W4Args a) {
-  const int cols = GLU ? a.N / 2 : a.N;
-  const long wide = (a.N + 15) / 16 * 16L, i = blockIdx.x * 256L + threadIdx.x;
-  wait_for_previous();
-  if (i >= (long)a.T * cols) return;
-  const int tok = (int)(i / cols), n = (int)(i % cols);
-  const float* p = a.parts + tok * wide + (GLU ? n / 8 * 16 + n % 8 : n);
-  float y = 0.f, up = 0.f;
-  for (int s = 0; s < a.slices; ++s, p += a.T * wide) {
-    y += p[0];
-    if (GLU) up += p[8];
-  }
-  if (GLU) y = y / (1.f + expf(-y)) * up;
-  if (a.residual) y += __bfloat162float(a.residual[(long)tok * a.r_tok + n]);
-  a.out[i] = __float2bfloat16(y);
 }
 
 __device__ __forceinline__ void cp16(void* dst, const void* src) {
@@ -403,7 +345,7 @@ int smem_of(int T, int units, bool whole, int nt) {
          (whole ? 0 : 2 * kWarps * 16 * (nt * 8 + 1) * 4);
 }
 
-int tiles_of_x(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : T <= 32 ? 4 : 8; }
+int tiles_of_x(int T) { return T <= 8 ? 1 : 2; }
 int units_of(const W4Args& a) {
   const int bu = blocks_of(tiles_of_x(a.T)), all = (a.K / 128 + bu - 1) / bu;
   return (all + a.slices - 1) / a.slices;
@@ -472,15 +414,21 @@ int run_group(const W4Args& a, int group, bool glu, int ctas, cudaStream_t st) {
 
 }  // namespace
 
-long linear_w4_work(int T, int N, int K, int sms) {
+long linear_w4_work(int T, int N, int K, int glu, int sms) {
   if (T < 1 || T > 64 || bad_shape(N, K, 32)) return 0;
+  const long wide = (N + 15) / 16 * 16L;
+  if (T > kFew) {
+    const int slices = wide_slices(T, N, K, sms);
+    return slices > 1 || glu ? slices * T * wide : 0;
+  }
   W4Args a{};
   a.T = T, a.N = N, a.K = K;
-  return plan(a, sms) == 0 || a.slices == 1 ? 0 : (long)a.slices * T * ((N + 15) / 16 * 16L);
+  return plan(a, sms) == 0 || a.slices == 1 ? 0 : (long)a.slices * T * wide;
 }
 
 int launch_linear_w4(const void* x, long x_tok, const void* codes, const void* scales, const void* residual, long r_tok,
-                     void* out, int T, int N, int K, int group, int glu, int sms, float* work, cudaStream_t st) {
+                     void* out, int T, int N, int K, int group, int glu, int sms, float* work, int* err,
+                     cudaStream_t st) {
   if (bad_shape(N, K, group) || T > 64 || (glu && N % (2 * kGlu))) return kErrBadArgsHost;
   if (T < 1) return 0;
   W4Args a{};
@@ -489,14 +437,13 @@ int launch_linear_w4(const void* x, long x_tok, const void* codes, const void* s
   a.residual = (const __nv_bfloat16*)residual, a.r_tok = r_tok;
   a.out = (__nv_bfloat16*)out, a.parts = work;
   a.T = T, a.N = N, a.K = K;
+  if (T > kFew) {
+    a.slices = wide_slices(T, N, K, sms);
+    return launch_wide(a, group, glu, err, st);
+  }
   const int ctas = plan(a, sms);
   if (ctas == 0) return kErrBadArgsHost;
-  switch (tiles_of_x(T)) {
-    case 1: return run_group<1>(a, group, glu, ctas, st);
-    case 2: return run_group<2>(a, group, glu, ctas, st);
-    case 4: return run_group<4>(a, group, glu, ctas, st);
-    default: return run_group<8>(a, group, glu, ctas, st);
-  }
+  return T <= 8 ? run_group<1>(a, group, glu, ctas, st) : run_group<2>(a, group, glu, ctas, st);
 }
 
 int launch_dequant_w4(const void* codes, const void* scales, void* out, int N, int K, int group, cudaStream_t st) {

@@ -13,7 +13,7 @@ import math
 import torch
 
 from . import gemm as G
-from ._ext import ext
+from ._ext import err_flag, ext
 
 BF16 = torch.bfloat16
 F32 = torch.float32
