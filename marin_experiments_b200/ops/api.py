@@ -311,5 +311,5 @@ def linear_w4(x, codes, scales, *, residual=None, glu: bool = False) -> torch.Te
         return R.linear_w4(x, codes, scales, residual, glu)
     if x.shape[0] <= 64:
         fns = _cuda()
-        return fns.ext().linear_w4(x, codes, scales, residual, glu, fns.err_flag(x.device) if x.shape[0] > 16 else None)
+        return fns.ext().linear_w4(x, codes, scales, residual, glu, fns.err_flag(x.device) if x.shape[0] > 32 else None)
     return _cuda().linear_w4_dense(x, codes, scales, residual, glu)

@@ -216,7 +216,7 @@ int launch_kv8_attention(const Kv8Cache& c, const Kv8Attention& a, cudaStream_t 
 // ----------------------------------------------------------------------- 4-bit weights (w4.cu)
 int launch_linear_w4(const void* x, long x_tok, const void* codes, const void* scales, const void* residual, long r_tok,
                      void* out, int T, int N, int K, int group, int glu, int sms, float* work, int* err,
-                     cudaStream_t st);  // err: set where a wait gave up (17 rows and more)
+                     cudaStream_t st);  // err: set where a wait gave up (33 rows and more)
 long linear_w4_work(int T, int N, int K, int glu, int sms);  // floats of its workspace
 int launch_dequant_w4(const void* codes, const void* scales, void* out, int N, int K, int group, cudaStream_t st);
 

@@ -747,8 +747,8 @@ Tensor linear_w4(const Tensor& x, const Tensor& codes, const Tensor& scales, con
   const at::AutoDispatchBelowADInplaceOrView plain;
   Tensor out = at::empty({x.size(0), glu ? N / 2 : N}, x.options()), work;
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  if (x.size(0) > 16) {
-    need(err.has_value(), "linear_w4 needs the device's error flag from 17 rows on");
+  if (x.size(0) > 32) {
+    need(err.has_value(), "linear_w4 needs the device's error flag from 33 rows on");
     cuda_i32(*err, "err");
     same_device(codes, {&*err});
   }

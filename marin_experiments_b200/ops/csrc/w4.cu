@@ -1,5 +1,5 @@
 // Products with 4-bit weights: y[t, n] = sum_k x[t, k] * code[n, k] * scale[n, k / group], for the few
-// rows (1 to 64) of a decode step, with the residual added or the SwiGLU applied before the one
+// rows (1 to 32; w4_wide.cu has 33 to 64) of a decode step, with the residual added or the SwiGLU applied before the one
 // rounding to bf16.
 //
 // Layout: int32 words [N][K / 8]. Within each 128 values of a row word 4 t + i of the 16 holds values
@@ -32,7 +32,7 @@ namespace mxk {
 namespace {
 
 constexpr int kWarps = 16;
-constexpr int kFew = 16;    // rows of x that these kernels take; w4_wide.cu takes more
+constexpr int kFew = 32;    // rows of x that these kernels take; w4_wide.cu takes more (times of both there)
 constexpr int kStages = 2;  // units of a warp on their way
 // Blocks of 128 values of K in a unit: 256 bytes of a row, or 128 where x needs the shared memory.
 __host__ __device__ constexpr int blocks_of(int nt) { return nt == 1 ? 4 : 2; }
@@ -345,7 +345,7 @@ int smem_of(int T, int units, bool whole, int nt) {
          (whole ? 0 : 2 * kWarps * 16 * (nt * 8 + 1) * 4);
 }
 
-int tiles_of_x(int T) { return T <= 8 ? 1 : 2; }
+int tiles_of_x(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : 4; }
 int units_of(const W4Args& a) {
   const int bu = blocks_of(tiles_of_x(a.T)), all = (a.K / 128 + bu - 1) / bu;
   return (all + a.slices - 1) / a.slices;
@@ -443,7 +443,11 @@ int launch_linear_w4(const void* x, long x_tok, const void* codes, const void* s
   }
   const int ctas = plan(a, sms);
   if (ctas == 0) return kErrBadArgsHost;
-  return T <= 8 ? run_group<1>(a, group, glu, ctas, st) : run_group<2>(a, group, glu, ctas, st);
+  switch (tiles_of_x(T)) {
+    case 1: return run_group<1>(a, group, glu, ctas, st);
+    case 2: return run_group<2>(a, group, glu, ctas, st);
+    default: return run_group<4>(a, group, glu, ctas, st);
+  }
 }
 
 int launch_dequant_w4(const void* codes, const void* scales, void* out, int N, int K, int group, cudaStream_t st) {

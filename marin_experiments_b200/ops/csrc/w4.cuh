@@ -37,7 +37,6 @@ __device__ __forceinline__ uint32_t pair_of(uint32_t w, int j, uint32_t magic, u
   return d;
 }
 
-
 // One output of a tile's row r (with GLU a unit, whose gate is y), or this slice's part of it.
 template <bool GLU>
 __device__ __forceinline__ void store(const W4Args& a, int slice, int tile, int r, int tok, float y, float up) {
@@ -75,7 +74,7 @@ __global__ void __launch_bounds__(256) slices_kernel(const __grid_constant__ W4A
 
 }  // namespace
 
-// Products of 17 to 64 rows of x (w4_wide.cu): CTAs' slices of K for these sizes, and the launch.
+// Products of 33 to 64 rows of x (w4_wide.cu): CTAs' slices of K for these sizes, and the launch.
 int wide_slices(int T, int N, int K, int sms);
 int launch_wide(const W4Args& a, int group, bool glu, int* err, cudaStream_t st);
 

@@ -1,4 +1,4 @@
-// 4-bit products of 17 to 64 rows on the tcgen05 tensor cores.
+// 4-bit products of 33 to 64 rows on the tcgen05 tensor cores.
 //
 // A CTA takes 128 rows of W and a slice of K. Eight warps turn the words into bf16 codes (exact, no
 // scale) and write them as the K-major 128-byte-swizzled A operand; x comes by TMA as B; one thread
@@ -6,10 +6,18 @@
 // TMEM, and four warps, a row of W a thread, add them to fp32 registers times the group's scale: as
 // exact as the kernel for fewer rows, where a scale folded into bf16 operands would round each weight.
 //
-// What bounds it: shared memory. A stage's codes are four times the words (32 KB written and read
-// again by the tensor core for 8 KB of weights), about twice the time that the words take from memory.
-// mma.sync bounded the kernel for fewer rows here: 40 products of m16n8k16 for 33 rows and 2048 weights
-// (33 rows, 4096 x 12288, groups of 32: 30 us).
+// What bounds it: the steps of a stage, each a wait of a warp: codes written, a fence, products issued,
+// sums read, about 0.45 us with four stages in flight. Without the products, the stores, the loads or the
+// sums it is 2 to 13 % faster, without all of them 30 %. More warps for the codes (16: 33 us where 8 take
+// 22), two issuing warps, stages of 256 values and a fifth stage were no faster. One thread found by
+// elect.sync with descriptors built once issues 20 % faster than lane 0 with descriptors built each time.
+//
+// The kernel for fewer rows (mma.sync) against this one, B200, device time in us:
+//   rows, N x K, group      mma.sync  this      rows, N x K, group      mma.sync  this
+//   32, 4096 x 4096, 128        11.9  10.5      33, 4096 x 12288, 32        30.0  21.1
+//   32, 24576 x 4096, 128       34.2    44      64, 4096 x 12288, 128       36.8  22.5
+//   32, 4096 x 12288, 32        21.2    21      64, 24576 x 4096, 64        76.6  53.1
+// so up to 32 rows, where mma.sync needs four products for 128 weights, stay there.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -32,17 +40,34 @@ namespace {
 
 constexpr int kRowsW = 128;              // rows of W of a CTA: M of the MMA
 constexpr int kStages = 4;
-constexpr int kSlots = 2;                // accumulators of a stage, used while the next fill
 constexpr int kCodeWarps = 8, kSumWarps = 4;
-constexpr int kThreads = 32 * (2 + kCodeWarps + kSumWarps);
+constexpr int kCodes0 = 2, kSums0 = kCodes0 + kCodeWarps;
+constexpr int kAhead = 4;                // stages whose words are loaded ahead
+constexpr int kThreads = 32 * (kSums0 + kSumWarps);
 constexpr int kABytes = kRowsW * 256;    // two tiles of 64 values of K
 constexpr int kErrX = 61, kErrCodes = 62, kErrMma = 63, kErrSums = 64;
 
 __host__ __device__ constexpr int stage_bytes(int n) { return kABytes + n * 256; }
 __host__ __device__ constexpr int acc_cols(int n) { return n <= 32 ? 32 : 64; }  // of one scale group
+// Accumulators of a stage, used while the next fill.
+__host__ __device__ constexpr int slots(int n, int gw) { return 4 * (4 / gw) * acc_cols(n) <= 512 ? 4 : 2; }
 __host__ __device__ constexpr int tmem_cols(int n, int gw) {
-  const int need = kSlots * (4 / gw) * acc_cols(n);
+  const int need = slots(n, gw) * (4 / gw) * acc_cols(n);
   return need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// a += x f in two sums by one instruction.
+__device__ __forceinline__ void fma2(float& a0, float& a1, float x0, float x1, float f) {
+  asm("{\n\t.reg .b64 a, x, g;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 x, {%2, %3};\n\tmov.b64 g, {%4, %4};\n\t"
+      "fma.rn.f32x2 a, x, g, a;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(x0), "f"(x1), "f"(f));
 }
 
 // The scales of a row in a stage.
@@ -72,6 +97,7 @@ template <int N, int GW, bool GLU>
 __global__ void __launch_bounds__(kThreads, 1)
     wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ W4Args a, int* err) {
   constexpr int G = 4 / GW;  // scale groups of a stage
+  constexpr int kSlots = slots(N, GW);
   constexpr uint32_t kCols = tmem_cols(N, GW);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -90,7 +116,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int d = 0; d < kSlots; ++d) {
       mbar_init(&sum_full[d], 1);
-      mbar_init(&sum_empty[d], 32 * kSumWarps);
+      mbar_init(&sum_empty[d], kSumWarps);
     }
     mbar_init(&drain, 1);
     fence_barrier_init();
@@ -126,9 +152,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         while (clock64() - t0 < (1ll << 24)) {}
       }
     }
-  } else if (warp == 1) {  // products
-    if (lane == 0) {
+  } else if (warp < kCodes0) {  // products
+    if (elect_one()) {
       constexpr uint32_t idesc = make_idesc_bf16(kRowsW, N, false, false);
+      const uint64_t codes0 = make_sdesc(smem_u32(smem), 16, 1024), x0 = codes0 + kABytes / 16;
       bool ok = true, issued = false;
       for (int it = 0; it < n_stages; ++it) {
         const int s = it % kStages, d = it % kSlots;
@@ -136,13 +163,12 @@ __global__ void __launch_bounds__(kThreads, 1)
              mbar_wait(&full[s], (it / kStages) & 1, err, kErrMma, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t codes = smem_u32(smem + s * stage_bytes(N)), x = codes + kABytes;
+        const uint64_t codes = codes0 + (uint32_t)(s * stage_bytes(N) / 16), x = x0 + (uint32_t)(s * stage_bytes(N) / 16);
+        const uint32_t to = tmem + d * G * acc_cols(N);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {  // 16 values of K
-          const uint64_t ad = make_sdesc(codes + (k / 4) * (kRowsW * 128) + (k % 4) * 32, 16, 1024);
-          const uint64_t bd = make_sdesc(x + (k / 4) * (N * 128) + (k % 4) * 32, 16, 1024);
-          umma_bf16(tmem + (d * G + k / (2 * GW)) * acc_cols(N), ad, bd, idesc, k % (2 * GW) != 0 ? 1u : 0u);
-        }
+        for (int k = 0; k < 8; ++k)  // 16 values of K
+          umma_bf16(to + k / (2 * GW) * acc_cols(N), codes + ((k / 4) * (kRowsW * 128) + (k % 4) * 32) / 16,
+                    x + ((k / 4) * (N * 128) + (k % 4) * 32) / 16, idesc, k % (2 * GW) != 0 ? 1u : 0u);
         issued = true;
         umma_commit(&empty[s]);
         umma_commit(&sum_full[d]);
@@ -153,10 +179,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         while (!mbar_try_wait(&drain, 0) && clock64() - t0 < (1ll << 26)) {}
       }
     }
-  } else if (warp < 2 + kCodeWarps) {  // codes
+  } else if (warp < kSums0) {  // codes
     // A thread has a quarter (16 bytes of words) of a block in rows r and r + 64. Rows of eight lanes
     // differ in bit 2, so that their swizzled 16-byte columns are all of the 128-byte row.
-    const int id = threadIdx.x - 64, t = id & 3, q = id >> 2;
+    const int id = threadIdx.x - 32 * kCodes0, t = id & 3, q = id >> 2;
     const int r = (q & ~7) | (q & 1) << 2 | (q >> 1 & 3);
     const uint32_t* p[2];
 #pragma unroll
@@ -170,30 +196,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         w[k][i] = k < n_stages ? __ldg(reinterpret_cast<const uint4*>(p[i] + k * 16)) : make_uint4(0, 0, 0, 0);
     uint32_t magic = 0x43004300u, bias = 0x43084308u;
     asm volatile("" : "+r"(magic), "+r"(bias));
-    for (int it = 0; it < n_stages; ++it) {
-      const int s = it % kStages;
-      const bool mine = lane != 0 || mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, err, kErrCodes, abort_flag);
-      if (!__all_sync(0xffffffffu, mine)) break;
-      uint8_t* dst = smem + s * stage_bytes(N);
+    bool mine = true;
+    for (int first = 0; first < n_stages && mine; first += kAhead) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t words[4] = {w[0][i].x, w[0][i].y, w[0][i].z, w[0][i].w};
+      for (int j = 0; j < kAhead; ++j) {  // unrolled: moving a register waits for the load that fills it
+        const int it = first + j, s = it % kStages;
+        if (it >= n_stages) break;
+        mine = lane != 0 || mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, err, kErrCodes, abort_flag);
+        mine = __all_sync(0xffffffffu, mine);
+        if (!mine) break;
+        uint8_t* dst = smem + s * stage_bytes(N);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {  // values 32 k + 8 t .. + 7
-          const int row = r + 64 * i, c = (k & 1) * 4 + t;
-          *reinterpret_cast<uint4*>(dst + (k >> 1) * (kRowsW * 128) + row * 128 + ((c ^ (row & 7)) << 4)) =
-              make_uint4(pair_of(words[k], 0, magic, bias), pair_of(words[k], 1, magic, bias),
-                         pair_of(words[k], 2, magic, bias), pair_of(words[k], 3, magic, bias));
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t words[4] = {w[j][i].x, w[j][i].y, w[j][i].z, w[j][i].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // values 32 k + 8 t .. + 7
+            const int row = r + 64 * i, c = (k & 1) * 4 + t;
+            *reinterpret_cast<uint4*>(dst + (k >> 1) * (kRowsW * 128) + row * 128 + ((c ^ (row & 7)) << 4)) =
+                make_uint4(pair_of(words[k], 0, magic, bias), pair_of(words[k], 1, magic, bias),
+                           pair_of(words[k], 2, magic, bias), pair_of(words[k], 3, magic, bias));
+          }
+          if (it + kAhead < n_stages) w[j][i] = __ldg(reinterpret_cast<const uint4*>(p[i] + (it + kAhead) * 16));
         }
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&full[s]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int k = 0; k + 1 < kAhead; ++k) w[k][i] = w[k + 1][i];
-        if (it + kAhead < n_stages) w[kAhead - 1][i] = __ldg(reinterpret_cast<const uint4*>(p[i] + (it + kAhead) * 16));
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[s]);
       }
     }
   } else {  // sums: one row of W a thread
@@ -210,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int d = it % kSlots;
       const RowScales<GW> sc = next;
       if (it + 1 < n_stages) next = sp[it + 1];
-      ok = mbar_wait(&sum_full[d], (it / kSlots) & 1, err, kErrSums, abort_flag);
+      ok = lane != 0 || mbar_wait(&sum_full[d], (it / kSlots) & 1, err, kErrSums, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
 #pragma unroll
@@ -223,11 +250,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld16(at + c, v);
           tmem_wait_ld();
 #pragma unroll
-          for (int n = 0; n < 16; ++n) acc[c + n] = fmaf(v[n], f, acc[c + n]);
+          for (int n = 0; n < 16; n += 2) fma2(acc[c + n], acc[c + n + 1], v[n], v[n + 1], f);
         }
       }
       tc_fence_before();
-      mbar_arrive(&sum_empty[d]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sum_empty[d]);
     }
     if (row < a.N) {
       if (a.slices > 1 || GLU) {
