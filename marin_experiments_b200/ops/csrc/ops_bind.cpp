@@ -584,7 +584,18 @@ std::vector<Tensor> block_tables_extend(const Tensor& tables, const Tensor& lens
                                      (int)free_pages.numel(), free_count.data_ptr<int>(), (int)page, (int)rows, b,
                                      b + R, b + R + 1, sl, sl + rows, sl + 2 * rows, sl + 3 * rows, stream()),
      "block_tables_extend");
-  return buf.split_with_sizes({R, 1, R + 1, rows, rows, rows, 1});
+  // Made by hand: split_with_sizes took 1 us more of the host's 9.
+  std::vector<Tensor> parts;
+  parts.reserve(7);
+  int64_t first = 0;
+  for (const int64_t n : {R, (int64_t)1, R + 1, rows, rows, rows, (int64_t)1}) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), buf.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(first);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(c10::IntArrayRef(n));
+    parts.push_back(std::move(t));
+    first += n;
+  }
+  return parts;
 }
 
 Tensor block_tables_release(const Tensor& tables, const Tensor& lens, const Tensor& done, const Tensor& free_pages,

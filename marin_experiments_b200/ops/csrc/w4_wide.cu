@@ -62,6 +62,10 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
 // a += x f in two sums by one instruction.
 __device__ __forceinline__ void fma2(float& a0, float& a1, float x0, float x1, float f) {
   asm("{\n\t.reg .b64 a, x, g;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 x, {%2, %3};\n\tmov.b64 g, {%4, %4};\n\t"
@@ -100,7 +104,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kSlots = slots(N, GW);
   constexpr uint32_t kCols = tmem_cols(N, GW);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);  // a cast of the address would make generic stores
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages], sum_full[kSlots], sum_empty[kSlots], drain;
   __shared__ uint32_t tmem_slot;
   __shared__ int aborted;
@@ -196,6 +200,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         w[k][i] = k < n_stages ? __ldg(reinterpret_cast<const uint4*>(p[i] + k * 16)) : make_uint4(0, 0, 0, 0);
     uint32_t magic = 0x43004300u, bias = 0x43084308u;
     asm volatile("" : "+r"(magic), "+r"(bias));
+    // Column 4 (k & 1) + t of the row's eight; rows 64 apart have the same swizzle.
+    const uint32_t mine_at = smem_u32(smem) + r * 128 + ((t ^ (r & 7)) << 4);
     bool mine = true;
     for (int first = 0; first < n_stages && mine; first += kAhead) {
 #pragma unroll
@@ -205,16 +211,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         mine = lane != 0 || mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, err, kErrCodes, abort_flag);
         mine = __all_sync(0xffffffffu, mine);
         if (!mine) break;
-        uint8_t* dst = smem + s * stage_bytes(N);
+        const uint32_t dst = mine_at + s * stage_bytes(N);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t words[4] = {w[j][i].x, w[j][i].y, w[j][i].z, w[j][i].w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {  // values 32 k + 8 t .. + 7
-            const int row = r + 64 * i, c = (k & 1) * 4 + t;
-            *reinterpret_cast<uint4*>(dst + (k >> 1) * (kRowsW * 128) + row * 128 + ((c ^ (row & 7)) << 4)) =
-                make_uint4(pair_of(words[k], 0, magic, bias), pair_of(words[k], 1, magic, bias),
-                           pair_of(words[k], 2, magic, bias), pair_of(words[k], 3, magic, bias));
+            sts128((k & 1 ? dst ^ 64 : dst) + (k >> 1) * (kRowsW * 128) + i * 64 * 128,
+                   pair_of(words[k], 0, magic, bias), pair_of(words[k], 1, magic, bias),
+                   pair_of(words[k], 2, magic, bias), pair_of(words[k], 3, magic, bias));
           }
           if (it + kAhead < n_stages) w[j][i] = __ldg(reinterpret_cast<const uint4*>(p[i] + (it + kAhead) * 16));
         }
