@@ -745,7 +745,7 @@ Tensor linear_w4(const Tensor& x, const Tensor& codes, const Tensor& scales, con
     TORCH_CHECK(s >= 0 && s % align == 0, n, ": the row stride must be a multiple of ", std::to_string(align));
     return (long)s;
   };
-  const long xt = rows(x, K, 8, "x");
+  long xt = rows(x, K, 8, "x");
   aligned16(x, "x");
   need(x.size(0) <= 64, "linear_w4 takes up to 64 rows");
   need(!glu || (N % 256 == 0 && !residual.has_value()), "glu: rows in blocks of 128 gate and 128 up, and no residual");
@@ -758,6 +758,11 @@ Tensor linear_w4(const Tensor& x, const Tensor& codes, const Tensor& scales, con
   const at::AutoDispatchBelowADInplaceOrView plain;
   Tensor out = at::empty({x.size(0), glu ? N / 2 : N}, x.options()), work;
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  Tensor apart;  // a TMA map wants rows that do not overlap, as those of an expanded x do
+  if (x.size(0) > 32 && xt < K) {
+    apart = x.contiguous();
+    xt = K;
+  }
   if (x.size(0) > 32) {
     need(err.has_value(), "linear_w4 needs the device's error flag from 33 rows on");
     cuda_i32(*err, "err");
@@ -765,7 +770,7 @@ Tensor linear_w4(const Tensor& x, const Tensor& codes, const Tensor& scales, con
   }
   const long floats = mxk::linear_w4_work((int)x.size(0), (int)N, (int)K, glu, sms);
   if (floats) work = at::empty({floats}, x.options().dtype(at::kFloat));
-  ok(mxk::launch_linear_w4(x.data_ptr(), xt, codes.data_ptr(), scales.data_ptr(), ptr<const void>(residual), rt,
+  ok(mxk::launch_linear_w4(apart.defined() ? apart.data_ptr() : x.data_ptr(), xt, codes.data_ptr(), scales.data_ptr(), ptr<const void>(residual), rt,
                            out.data_ptr(), (int)x.size(0), (int)N, (int)K, group, glu, sms,
                            floats ? work.data_ptr<float>() : nullptr, ptr<int>(err), stream()),
      "linear_w4");

@@ -48,13 +48,10 @@ constexpr int kABytes = kRowsW * 256;    // two tiles of 64 values of K
 constexpr int kErrX = 61, kErrCodes = 62, kErrMma = 63, kErrSums = 64;
 
 __host__ __device__ constexpr int stage_bytes(int n) { return kABytes + n * 256; }
-__host__ __device__ constexpr int acc_cols(int n) { return n <= 32 ? 32 : 64; }  // of one scale group
+constexpr int kAccCols = 64;             // of one scale group's accumulator
 // Accumulators of a stage, used while the next fill.
-__host__ __device__ constexpr int slots(int n, int gw) { return 4 * (4 / gw) * acc_cols(n) <= 512 ? 4 : 2; }
-__host__ __device__ constexpr int tmem_cols(int n, int gw) {
-  const int need = slots(n, gw) * (4 / gw) * acc_cols(n);
-  return need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
-}
+__host__ __device__ constexpr int slots(int gw) { return 4 * (4 / gw) * kAccCols <= 512 ? 4 : 2; }
+__host__ __device__ constexpr int tmem_cols(int gw) { return slots(gw) * (4 / gw) * kAccCols; }  // 256 or 512
 
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -101,8 +98,8 @@ template <int N, int GW, bool GLU>
 __global__ void __launch_bounds__(kThreads, 1)
     wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ W4Args a, int* err) {
   constexpr int G = 4 / GW;  // scale groups of a stage
-  constexpr int kSlots = slots(N, GW);
-  constexpr uint32_t kCols = tmem_cols(N, GW);
+  constexpr int kSlots = slots(GW);
+  constexpr uint32_t kCols = tmem_cols(GW);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);  // a cast of the address would make generic stores
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages], sum_full[kSlots], sum_empty[kSlots], drain;
@@ -168,10 +165,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         tc_fence_after();
         const uint64_t codes = codes0 + (uint32_t)(s * stage_bytes(N) / 16), x = x0 + (uint32_t)(s * stage_bytes(N) / 16);
-        const uint32_t to = tmem + d * G * acc_cols(N);
+        const uint32_t to = tmem + d * G * kAccCols;
 #pragma unroll
         for (int k = 0; k < 8; ++k)  // 16 values of K
-          umma_bf16(to + k / (2 * GW) * acc_cols(N), codes + ((k / 4) * (kRowsW * 128) + (k % 4) * 32) / 16,
+          umma_bf16(to + k / (2 * GW) * kAccCols, codes + ((k / 4) * (kRowsW * 128) + (k % 4) * 32) / 16,
                     x + ((k / 4) * (N * 128) + (k % 4) * 32) / 16, idesc, k % (2 * GW) != 0 ? 1u : 0u);
         issued = true;
         umma_commit(&empty[s]);
@@ -248,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) {
         const float f = sc.at(gi);
-        const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16) + (d * G + gi) * acc_cols(N);
+        const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16) + (d * G + gi) * kAccCols;
 #pragma unroll
         for (int c = 0; c < N; c += 16) {
           float v[16];
@@ -347,7 +344,6 @@ int wide_slices(int T, int N, int K, int sms) {
 
 int launch_wide(const W4Args& a, int group, bool glu, int* err, cudaStream_t st) {
   if (err == nullptr || (glu && a.parts == nullptr)) return kErrBadArgsHost;
-  if (a.T <= 32) return run_group<32>(a, group, glu, err, st);
   if (a.T <= 48) return run_group<48>(a, group, glu, err, st);
   return run_group<64>(a, group, glu, err, st);
 }

@@ -428,6 +428,55 @@ def test_linear_w4_beyond_32_bit_offsets():
     O.close(got[:, -1000:], y, O.w4_bound(y, size, k))
 
 
+@pytest.mark.parametrize("t", [8, 40, 70])
+def test_linear_w4_of_one_row_repeated(t):
+    """An expanded x (row stride 0) gives what its copy gives."""
+    _, packed, scales, x = w4_case(200, 1024, 64, 1)
+    c, s, x = packed.cuda(), scales.cuda(), x.cuda().expand(t, -1)
+    got = api.linear_w4(x, c, s)
+    assert torch.equal(got, api.linear_w4(x.contiguous(), c, s))
+    assert (got == got[0]).all()
+
+
+@pytest.mark.parametrize("t", [16, 33, 48, 49, 64])
+def test_linear_w4_rows_do_not_mix(t):
+    """A NaN in one row of x reaches that row's results alone, and the others keep their bits."""
+    _, packed, scales, x = w4_case(300, 2048, 32, t)
+    c, s, x = packed.cuda(), scales.cuda(), x.cuda()
+    clean = api.linear_w4(x, c, s)
+    x[t // 2, 700] = float("nan")
+    got = api.linear_w4(x, c, s)
+    assert got[t // 2].isnan().all()
+    got[t // 2] = clean[t // 2]
+    assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("t", [4, 40])
+def test_linear_w4_in_two_graphs_and_streams(t):
+    """Graphs with split sums replay beside one another and beside an eager call."""
+    _, packed, scales, _ = w4_case(512, 12288, 32, t)
+    c, s = packed.cuda(), scales.cuda()
+    x = [torch.randn(t, 12288, device="cuda").to(BF16) for _ in range(3)]
+    want = [api.linear_w4(v, c, s) for v in x]
+    graphs, outs = [], []
+    for v in x[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(api.linear_w4(v, c, s))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            third = api.linear_w4(x[2], c, s)
+    torch.cuda.synchronize()
+    for got, w in zip([*outs, third], want):
+        assert torch.equal(got, w)
+
+
 def test_linear_w4_nan_scale_shows():
     w = torch.randn(32, 256)
     w[5, 130] = float("inf")
