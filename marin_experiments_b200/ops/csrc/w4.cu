@@ -184,7 +184,9 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
   for (int i = tid; i < 2 * kWarps; i += kThreads) part_tile[i] = -1;
   // launched early: the kernel before may still be writing x (or the weights)
   wait_for_previous();
-  if (a.slices > 1) let_next_start();
+  // The next kernel's CTAs may take this kernel's places as they come free, and do there what needs no
+  // memory (4096 x 4096, one row, in a row: 4.85 -> 4.56 us a product; 24576 x 4096, 16 rows: 22.4 -> 21.3).
+  let_next_start();
   // x before the weights, which would keep the memory busy for longer than it waits.
   // Blocks that the last unit lacks meet zeros (their codes are what the ring held).
   for (int c = tid; c < units * BU * 16; c += kThreads) {

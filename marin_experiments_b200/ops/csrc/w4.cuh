@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(256) slices_kernel(const __grid_constant__ W4A
   const int cols = GLU ? a.N / 2 : a.N;
   const long wide = (a.N + 15) / 16 * 16L, i = blockIdx.x * 256L + threadIdx.x;
   wait_for_previous();
+  let_next_start();
   if (i >= (long)a.T * cols) return;
   const int tok = (int)(i / cols), n = (int)(i % cols);
   const float* p = a.parts + tok * wide + (GLU ? n / 8 * 16 + n % 8 : n);

@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   wait_for_previous();
-  if (a.slices > 1 || GLU) let_next_start();
+  let_next_start();
 
   if (warp == 0) {  // x
     if (lane == 0) {
