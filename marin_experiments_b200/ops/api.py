@@ -20,10 +20,17 @@ from .layout import split_gate_up
 from .quant import dequantize_w4, quantize_w4  # noqa: F401  (public names of the 4-bit weights)
 
 
-def _cuda():
-    from . import cuda_fns
+_CUDA = None
 
-    return cuda_fns
+
+def _cuda():
+    """``cuda_fns``, which needs the built extension; kept, as an import statement costs 0.6 us a call."""
+    global _CUDA
+    if _CUDA is None:
+        from . import cuda_fns
+
+        _CUDA = cuda_fns
+    return _CUDA
 
 
 # ---------------------------------------------------------------------------------- embedding
@@ -248,8 +255,8 @@ def block_tables_extend(tables, lens, new_lens, free_pages, free_count, page_siz
     the caller keeps the plan's ``lens`` and ``free_count`` when it takes the step. Up to 4096
     requests."""
     if tables.is_cuda:
-        return BlockPlan(*_cuda().ext().block_tables_extend(tables, lens, new_lens, free_pages, free_count, page_size,
-                                                            rows))
+        return BlockPlan._make(_cuda().ext().block_tables_extend(tables, lens, new_lens, free_pages, free_count,
+                                                                 page_size, rows))
     return BlockPlan(*R.block_tables_extend(tables, lens, new_lens, free_pages, free_count, page_size, rows))
 
 

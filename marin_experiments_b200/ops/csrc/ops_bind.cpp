@@ -2,6 +2,7 @@
 #include <algorithm>
 #include <string>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -554,6 +555,10 @@ void cuda_i32(const Tensor& t, const char* n) {
 void same_device(const Tensor& a, std::initializer_list<const Tensor*> rest) {
   for (auto* t : rest) TORCH_CHECK(t->device() == a.device(), "all tensors must be on one device");
 }
+// at::empty without the dispatcher: 0.2 us less on the host.
+Tensor fresh(c10::IntArrayRef sizes, const Tensor& on, at::ScalarType type) {
+  return at::detail::empty_cuda(sizes, type, on.device(), std::nullopt);
+}
 bool overlaps(const Tensor& a, const Tensor& b) {
   const char *x = (const char*)a.data_ptr(), *y = (const char*)b.data_ptr();
   return x < y + b.nbytes() && y < x + a.nbytes();
@@ -576,7 +581,7 @@ std::vector<Tensor> block_tables_extend(const Tensor& tables, const Tensor& lens
   c10::cuda::CUDAGuard g(tables.device());
   const at::AutoDispatchBelowADInplaceOrView plain;  // views without autograd's records
   // one buffer: lens [R], free_count, starts [R + 1], slots, requests, positions [rows], status
-  Tensor buf = at::empty({2 * R + 3 + 3 * rows}, tables.options());
+  Tensor buf = fresh({2 * R + 3 + 3 * rows}, tables, at::kInt);
   int* b = buf.data_ptr<int>();
   int* sl = b + 2 * R + 2;
   ok(mxk::launch_block_tables_extend(tables.data_ptr<int>(), (int)tables.size(1), lens.data_ptr<int>(),
@@ -613,7 +618,7 @@ Tensor block_tables_release(const Tensor& tables, const Tensor& lens, const Tens
        "page must be positive, and a table at most 2^30 tokens");
   c10::cuda::CUDAGuard g(tables.device());
   const at::AutoDispatchBelowADInplaceOrView plain;
-  Tensor status = at::empty({1}, tables.options());
+  Tensor status = fresh({1}, tables, at::kInt);
   ok(mxk::launch_block_tables_release(tables.data_ptr<int>(), (int)tables.size(1), lens.data_ptr<int>(),
                                       (const uint8_t*)done.data_ptr(), (int)R, free_pages.data_ptr<int>(),
                                       (int)free_pages.numel(), free_count.data_ptr<int>(), (int)page,
@@ -699,7 +704,7 @@ Tensor kv8_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const 
     need(o.sizes() == q.sizes(), "out must have q's shape");
     need(!overlaps(o, kc) && !overlaps(o, vc) && (T == 0 || !overlaps(o, q)), "out must not overlap an input");
   } else {
-    o = at::empty(q.sizes(), q.options());
+    o = fresh(q.sizes(), q, at::kBFloat16);
   }
   if (T == 0) return o;
   mxk::Kv8Attention a{q.data_ptr(), qt, tables.data_ptr<int>(), lens.data_ptr<int>(),
@@ -710,7 +715,7 @@ Tensor kv8_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const 
   const long floats = mxk::kv8_attention_work(a, c.hd);
   Tensor work;
   if (floats) {
-    work = at::empty({floats}, ks.options());
+    work = fresh({floats}, ks, at::kFloat);
     a.work = work.data_ptr<float>();
   }
   ok(mxk::launch_kv8_attention(c, a, stream()), "kv8_attention");
@@ -756,7 +761,7 @@ Tensor linear_w4(const Tensor& x, const Tensor& codes, const Tensor& scales, con
   }
   c10::cuda::CUDAGuard g(codes.device());
   const at::AutoDispatchBelowADInplaceOrView plain;
-  Tensor out = at::empty({x.size(0), glu ? N / 2 : N}, x.options()), work;
+  Tensor out = fresh({x.size(0), glu ? N / 2 : N}, x, at::kBFloat16), work;
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   Tensor apart;  // a TMA map wants rows that do not overlap, as those of an expanded x do
   if (x.size(0) > 32 && xt < K) {
@@ -769,7 +774,7 @@ Tensor linear_w4(const Tensor& x, const Tensor& codes, const Tensor& scales, con
     same_device(codes, {&*err});
   }
   const long floats = mxk::linear_w4_work((int)x.size(0), (int)N, (int)K, glu, sms);
-  if (floats) work = at::empty({floats}, x.options().dtype(at::kFloat));
+  if (floats) work = fresh({floats}, x, at::kFloat);
   ok(mxk::launch_linear_w4(apart.defined() ? apart.data_ptr() : x.data_ptr(), xt, codes.data_ptr(), scales.data_ptr(), ptr<const void>(residual), rt,
                            out.data_ptr(), (int)x.size(0), (int)N, (int)K, group, glu, sms,
                            floats ? work.data_ptr<float>() : nullptr, ptr<int>(err), stream()),
