@@ -50,7 +50,12 @@ constexpr int kJoinWarps = 8;
 // 32768 tokens: 254 us at 1 round, 249 at 2, 242 at 4, 237 at 8; 259 with 8 steps a CTA).
 constexpr long kRounds = 8;
 constexpr int kManySteps = 16;
-constexpr int kClusterSteps = 16;    // most steps a CTA of a cluster takes
+// Most steps that a CTA of a cluster takes. Where clusters leave more than half of the GPU's places free,
+// sharing the steps among all places is worth the join's launch from three steps on (us, in clusters and
+// shared; one request of 2000 tokens, 8 kv heads: 8.35, 7.7; of 4000: 9.5, 8.3; two of 4000: 11.7, 9.7;
+// 1000 tokens, two steps: 6.8, 7.1). Where they fill it, not (16 requests of 500 to 2000 tokens: 15.5,
+// 17.5; 24 of 7 to 6001, 2 kv heads: 11.1, 12.3).
+constexpr int kClusterSteps = 16, kFewClusterSteps = 2;
 
 // Chunks of a warp on their way, and CTAs an SM: what its registers hold without spilling (255 at
 // two, 168 at three, 128 at four), and 228 KB of shared memory hold of rings (a stage is 32 KB of a
@@ -874,7 +879,8 @@ bool kv8_attention_plan(Kv8Attention& a, int hkv, int page, int hd, int sms) {
   int size = 8;
   while (size > 1 && segs * size > at_once) size /= 2;
   while (size > 1 && size / 2 >= steps) size /= 2;
-  if (a.tile <= 16 && segs * size <= at_once && steps <= (long)kClusterSteps * size) {
+  const long most_steps = size * (long)(2 * segs * size <= ctas ? kFewClusterSteps : kClusterSteps);
+  if (a.tile <= 16 && segs * size <= at_once && steps <= most_steps) {
     a.cluster = size;
     a.grid = (int)(segs * size);
   } else {
