@@ -311,42 +311,51 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
   wait_for_previous();
   if (!CLUSTER) let_next_start();
 
-  // Steps (with CLUSTER segments) before each request, each thread's requests in a row. Ascending
-  // starts keep the sum below the host's bound; with any other nothing is computed.
-  const int per = (a.R + kThreads - 1) / kThreads;
-  auto weight = [&](int r, int& bad) {
-    int first;
-    const int n = new_rows(a, r, first);
-    if (a.starts != nullptr) bad |= a.starts[r + 1] < first;
-    return (n * rep + kRows - 1) / kRows * c.hkv * (CLUSTER ? 1 : steps_of(cap, a.lens[r]));
-  };
-  int mine = 0, bad = 0;
-  for (int i = 0; i < per; ++i)
-    if (tid * per + i < a.R) mine += weight(tid * per + i, bad);
-  int x = mine;
+  int total = 0, bad = 0;
+  // Segments of a request where all have one row: a cluster then knows its request without a sum over the
+  // others' (one request of 1000 tokens: 6.8 -> 6.6 us; 24 of 7 to 6001, 2 kv heads: 11.2 -> 10.4).
+  const int same = CLUSTER && a.starts == nullptr ? (rep + kRows - 1) / kRows * c.hkv : 0;
+  if (same) {
+    total = a.R * same;
+    __syncthreads();
+  } else {
+    // Steps (with CLUSTER segments) before each request, each thread's requests in a row. Ascending
+    // starts keep the sum below the host's bound; with any other nothing is computed.
+    const int per = (a.R + kThreads - 1) / kThreads;
+    auto weight = [&](int r, int& bad) {
+      int first;
+      const int n = new_rows(a, r, first);
+      if (a.starts != nullptr) bad |= a.starts[r + 1] < first;
+      return (n * rep + kRows - 1) / kRows * c.hkv * (CLUSTER ? 1 : steps_of(cap, a.lens[r]));
+    };
+    int mine = 0;
+    for (int i = 0; i < per; ++i)
+      if (tid * per + i < a.R) mine += weight(tid * per + i, bad);
+    int x = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += u;
-  }
-  if (lane == 31) warp_sums[warp] = x;
-  bad = __syncthreads_or(bad);
-  int before = x - mine, total = 0;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    if (i < warp) before += warp_sums[i];
-    total += warp_sums[i];
-  }
-  for (int i = 0; i < per; ++i) {
-    const int r = tid * per + i;
-    if (r < a.R) {
-      prefix[r] = before;
-      before += weight(r, bad);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += u;
     }
+    if (lane == 31) warp_sums[warp] = x;
+    bad = __syncthreads_or(bad);
+    int before = x - mine;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) before += warp_sums[i];
+      total += warp_sums[i];
+    }
+    for (int i = 0; i < per; ++i) {
+      const int r = tid * per + i;
+      if (r < a.R) {
+        prefix[r] = before;
+        if (i + 1 < per) before += weight(r, bad);
+      }
+    }
+    if (bad) total = 0;
+    if (tid == 0) prefix[a.R] = total;
+    __syncthreads();
   }
-  if (bad) total = 0;
-  if (tid == 0) prefix[a.R] = total;
-  __syncthreads();
   if (!CLUSTER && blockIdx.x == 0)
     for (int r = tid; r <= a.R; r += kThreads) w.prefix[r] = prefix[r];
   if (a.zero_tail) {  // rows of no request: before the first, behind the last, all if starts do not ascend
@@ -378,12 +387,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
   }
   const int begin = at;
   while (at < end) {
-    const int r = owner(prefix, a.R, at);
+    const int r = same ? at / same : owner(prefix, a.R, at);
     const int len_in = a.lens[r];
     int row0;
     const int n_new = new_rows(a, r, row0);
     const int steps = steps_of(cap, len_in);
-    const int in_r = at - prefix[r], seg = CLUSTER ? in_r : in_r / steps;  // segments of a request: row tiles x kv heads
+    const int in_r = at - (same ? r * same : prefix[r]), seg = CLUSTER ? in_r : in_r / steps;  // segments of a request: row tiles x kv heads
     const int tile = args.hkv.by(seg), kh = seg - tile * c.hkv;
     const int s0 = CLUSTER ? steps * rank / parts : in_r - seg * steps, seg_start = at - s0;
     const int s1 = CLUSTER ? steps * (rank + 1) / parts : min(steps, s0 + (end - at));
