@@ -101,9 +101,10 @@ __device__ __forceinline__ uint2 rescale8(uint2 u, float ratio) {
 // values are loaded while its length is still looked for (they are masked when it is known).
 constexpr int kAppendThreads = 256;
 constexpr int kAppendWarps = kAppendThreads / 32;
+constexpr int kManyRows = 64;  // of a window: a prompt's
 
 // Pages of 128 hold 8 pieces a thread: held to 3 CTAs an SM (16000 rows 24.3 -> 19.1 us then),
-// the others to 4 (7000 rows in pages of 64: 14.9 us; 23 at one, where registers are not held back).
+// the others to 4 (8000 rows in pages of 64 15 us then; 23 at one, where registers are not held back).
 template <int HD, int PAGE>
 __global__ void __launch_bounds__(kAppendThreads, PAGE == 128 ? 3 : 4)
     append_kernel(const __grid_constant__ Kv8Cache c, const __nv_bfloat16* __restrict__ k_new,
@@ -123,14 +124,23 @@ __global__ void __launch_bounds__(kAppendThreads, PAGE == 128 ? 3 : 4)
   const int limit = c.pages * PAGE;  // below 2^31 by the host's check
   wait_for_previous();
   const int stop = (int)min((long)rows, (at + 1L) * window);
-  for (int r0 = at * window; r0 < stop; r0 += 32) {
+  // A prompt's rows come to L2 while their slots are looked at (8000 rows 14.9 -> 13.5 us; a decode step's
+  // few are slower for it, 256 rows 3.75 -> 3.82).
+  constexpr int kLines = HD / 64;
+  if (window >= kManyRows)
+    for (int p = tid; p < (stop - at * window) * kLines; p += kAppendThreads)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(src + (at * window + p / kLines) * tok + p % kLines * 64));
+  int slot_ahead, prev_ahead;  // of this lane's row and the row before
+  auto look = [&](int r0) {
     const int row = r0 + lane;
+    slot_ahead = row < stop ? slots[row] : -1;
+    prev_ahead = row < stop && row > 0 ? slots[row - 1] : -2;
+  };
+  look(at * window);
+  for (int r0 = at * window; r0 < stop; r0 += 32) {
     // runs that start in these 32 rows
-    int slot = -1, prev = -2;
-    if (row < stop) {
-      slot = slots[row];
-      if (row > 0) prev = slots[row - 1];
-    }
+    const int slot = slot_ahead, prev = prev_ahead;
+    look(r0 + 32);
     const bool first = slot >= 0 && slot < limit && (slot % PAGE == 0 || prev != slot - 1);
     const uint32_t runs = __ballot_sync(0xffffffffu, first);
     const bool together = __popc(runs) <= 2;
@@ -232,8 +242,9 @@ int launch_kv8_append(const Kv8Cache& c, const void* k, const void* v, long k_to
   // Few rows are a decode step's, whose runs of one row want a warp each; many are a prompt's, whose runs
   // want a CTA each and no CTA without one (us at windows of 8, 16, 32, 64; 8 kv heads of 128 dims: 256
   // runs of a row 3.7, 4.7, 7.3, 13; a prompt of 700 rows 4.5, 3.7, 3.4, 3.6; 1000 runs of a row 10.5, 10.0,
-  // 10.3, 14; 7000 rows of prompts at 16, 32, 64, 128: 21, 15.9, 14.9, 15.6).
-  const int window = rows <= 256 ? 8 : rows <= 2048 ? 16 : 64;
+  // 10.3, 14; 8000 rows of prompts at 16, 32, 64, 128, before they were fetched ahead: 21, 15.9, 14.9,
+  // 15.6).
+  const int window = rows <= 256 ? 8 : rows <= 2048 ? 16 : kManyRows;
   if (c.hd == 64) return launch_append<64>(c, k, v, k_tok, v_tok, slots, rows, window, st);
   if (c.hd == 128) return launch_append<128>(c, k, v, k_tok, v_tok, slots, rows, window, st);
   return kErrBadArgsHost;
