@@ -13,9 +13,10 @@
 // exactly; x is bf16 as it stands; products and sums are fp32, and the scale multiplies the group's
 // fp32 sum.
 //
-// What bounds it: N * K / 2 bytes of weights against 2 * T * N * K operations, so memory for T up to
-// about 16, then the conversions and mma.sync's rate; at a few MB a matrix, the start and one round
-// trip to memory.
+// What bounds it: at 151936 x 4096 nearly the N * K / 2 bytes of weights (5.1 TB/s); else shared memory,
+// which gives 512 bytes of x to every 16 x 32 weights and takes and gives their words (64 weights a clock
+// and SM at most; 42 reached) next to the conversions' issue slots; at a few MB a matrix also the start
+// and one round trip to memory.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
