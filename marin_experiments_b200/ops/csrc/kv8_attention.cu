@@ -793,15 +793,20 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
   const int rep = args.rep.d;
   wait_for_previous();
   int r = row;
+  const int total = w.prefix[a.R];
+  if (total == 0) return;  // nothing was computed: starts that do not ascend, or no request has a row
   if (a.starts != nullptr) {
-    if (row >= a.starts[a.R]) return;
+    // Rows of no request. Before the first, row - starts[r] is negative: every index below would lie
+    // before its array.
+    if (row < a.starts[0] || row >= a.starts[a.R]) return;
     r = owner(a.starts, a.R, row);
   }
   int row0;
-  if (row - (a.starts ? a.starts[r] : r) >= new_rows(a, r, row0)) return;
-  const int total = w.prefix[a.R], start = w.prefix[r];
+  const int n_new = new_rows(a, r, row0);
+  if (row < row0 || row - row0 >= n_new) return;
+  const int start = w.prefix[r];
   const int steps = steps_of(a.width << args.page_shift, a.lens[r]);
-  if (steps == 1 || total == 0) return;  // one step has one CTA
+  if (steps == 1) return;  // one step has one CTA
   const int kh = args.rep.by(h), x = (row - row0) * rep + h - kh * rep, tile = x / a.tile, y = x % a.tile;
   const Share share(total, used_ctas(a, total));
   const int s0 = start + (tile * c.hkv + kh) * steps;
