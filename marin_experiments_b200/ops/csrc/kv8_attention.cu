@@ -12,7 +12,9 @@
 // that brings its largest value to 2^13, so its bf16 values are exact in f16 too (what is 2^-37 of
 // the row's largest rounds). Scores and sums are fp32. The weights p = 2^(s - max + 15) round to f16,
 // 2^-12 of a weight at most (below 2^-29 of the largest weight: absolutely). Output sums are held in
-// units of the current page's scale; a page of another scale rescales them by a power of two.
+// units of the current page's scale; a page of another scale rescales them by a power of two. The unit stays
+// above 2^-60 of the largest that a warp has met in the segment, so the weights of pages below 2^-89 of that lose
+// bits (2^15 * 2^-29 is f16's least normal number).
 //
 // A NaN value must reach the rows that see it and no other, but 0 * NaN would reach all rows of a
 // tile. append marks pages that hold a NaN value in the sign of v_scale; before such a page's values
@@ -511,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
       }
     }
 
-    float o[MT][NQ][4], m[NQ][2], l[NQ][2], unit = 0.f;
+    float o[MT][NQ][4], m[NQ][2], l[NQ][2], unit = 0.f, least = 0.f;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
 #pragma unroll
@@ -571,8 +573,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
       const bool diag = key0 + kChunk > min(len, tile_first + 1);  // some row does not see some key
       float pscale = 1.f, ratio = 1.f;
       const float v_unit = fabsf(vs);
-      if (v_unit != unit && v_unit > 0.f) {  // sums in units of this page's scale (2^-60 of the last at least)
-        const float now = fmaxf(v_unit, unit * 0x1p-60f);
+      if (v_unit != unit && v_unit > 0.f) {  // sums in units of this page's scale
+        // 2^-60 at least of the largest unit that the sums have had, however often it falls: a page of zeros
+        // has 2^-110, and the sums (2^15 * 448 a key) times all falls stay below 2^104 for 2^20 keys.
+        least = fmaxf(least, v_unit * 0x1p-60f);
+        const float now = fmaxf(v_unit, least);
         ratio = unit / now;
         pscale = v_unit / now;
         unit = now;

@@ -48,3 +48,83 @@ def test_attention_rows_before_the_first_request(h, hkv, hd, lens, new, lead, ta
     attend(q.cuda(), d, starts=ints(starts), out=out)
     assert bool((out[:lead] == 7).all()) and bool((out[starts[-1]:] == 7).all())
     assert torch.equal(out[lead:starts[-1]], got[lead:starts[-1]])
+
+
+def appended(lens, k, v, page):
+    """A cache that ``kv8_append`` wrote: request r holds the first ``lens[r]`` of the rows ``k[r]``,
+    ``v[r]`` ``[tokens, kv_heads, head_dim]``."""
+    hkv, hd = k.shape[2:]
+    need = [-(-n // page) for n in lens]
+    pages, width = sum(need), max(need)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(7)).int()
+    tables = torch.full((len(lens), width), -1, dtype=torch.int32)
+    at = 0
+    for r, n in enumerate(need):
+        tables[r, :n] = order[at:at + n]
+        at += n
+    c = {"k": torch.zeros(pages, hkv, page, hd, device="cuda").to(O.E4M3), "ks": torch.zeros(pages, hkv, device="cuda")}
+    c |= {"v": c["k"].clone(), "vs": c["ks"].clone(), "tables": tables.cuda(), "lens": ints(lens)}
+    for r, n in enumerate(lens):
+        t = torch.arange(n)
+        slots = tables[r, t // page] * page + t % page
+        api.kv8_append(k[r, :n].to(BF16).cuda(), v[r, :n].to(BF16).cuda(), c["k"], c["v"], c["ks"], c["vs"],
+                       slots.int().cuda())
+    return c
+
+
+# (requests, kv heads, tokens): long requests shared among all CTAs, a step of 128 keys each and many steps
+# each; clusters of 8 whose CTAs take three steps each; clusters of one CTA.
+SPLITS = [(2, 2, 5000), (40, 8, 3000), (4, 8, 3072), (37, 8, 1100)]
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("r,hkv,n", SPLITS)
+@pytest.mark.parametrize("first,zeros,mean,size", [(128, 256, 1.0, 1.0), (512, 512, 0.0, 4.0), (128, 256, 1.0, 1e4),
+                                                   (129, 900, 1.0, 1e-3)])
+def test_attention_behind_values_that_are_zero(hd, r, hkv, n, first, zeros, mean, size):
+    """Ordinary values, then hundreds of tokens whose values are all zero (their pages have the least
+    scale there is), then ordinary ones; again and again over the context."""
+    g = torch.Generator().manual_seed(3)
+    k = 0.3 * torch.randn(r, n, hkv, hd, generator=g)
+    v = size * (mean + torch.randn(r, n, hkv, hd, generator=g))
+    t = torch.arange(n)
+    v[:, t % (first + zeros) >= first] = 0
+    d = appended([n] * r, k, v, 64)
+    q = torch.randn(r, hkv, hd, generator=g).to(BF16)
+    want, s = O.attention64(q, {x: y.cpu() for x, y in d.items()})
+    O.close(attend(q.cuda(), d), want, O.attention_bound(want, s))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("r,hkv,n", SPLITS)
+@pytest.mark.parametrize("drop", [-20, -35, -45])
+def test_attention_over_scales_that_fall_again_and_again(hd, r, hkv, n, drop):
+    """Values of 2^0, 2^drop, 2^(2 drop) by turns of 128 tokens."""
+    g = torch.Generator().manual_seed(4)
+    k = 0.3 * torch.randn(r, n, hkv, hd, generator=g)
+    e = drop * (torch.arange(n) // 128 % 3)
+    v = (1 + torch.rand(r, n, hkv, hd, generator=g)) * torch.exp2(e.double()).float()[:, None, None]
+    d = appended([n] * r, k, v, 64)
+    q = torch.randn(r, hkv, hd, generator=g).to(BF16)
+    want, s = O.attention64(q, {x: y.cpu() for x, y in d.items()})
+    O.close(attend(q.cuda(), d), want, O.attention_bound(want, s))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("drop", [-8, -16, -28])
+def test_attention_of_small_values_behind_large_ones(hd, drop):
+    """The weight on values far smaller than those before them in the cache, which a fall of the sums'
+    unit by 2^56 in all must keep."""
+    g = torch.Generator().manual_seed(5)
+    n, hkv = 1536, 8
+    part = torch.arange(n) // 128 % 3
+    v = (1 + torch.rand(1, n, hkv, hd, generator=g)) * torch.exp2((drop * part).float())[:, None, None]
+    k = 0.02 * torch.randn(1, n, hkv, hd, generator=g)
+    k[..., 0] += torch.where(part == 2, 30.0, -30.0)[:, None]
+    q = torch.randn(1, hkv, hd, generator=g)
+    q[..., 0] = 40.0
+    d = appended([n], k, v, 64)
+    want, s = O.attention64(q.to(BF16), {x: y.cpu() for x, y in d.items()})
+    assert float(want.abs().max()) < 4 * 2.0 ** (2 * drop)
+    # the bound's 1e-30 stays below 2^-8 of the least of these values (2^-56)
+    O.close(attend(q.to(BF16).cuda(), d), want, O.attention_bound(want, s))
