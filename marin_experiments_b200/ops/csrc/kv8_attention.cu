@@ -149,6 +149,12 @@ __device__ __forceinline__ float part_weight(float m, float l, float mx) {
   return ex2(m - mx);
 }
 
+// The least power of two >= x, and the inverse of one (2^-126 to 2^126): divisions take longer.
+__device__ __forceinline__ float power_of_two(float x) {
+  return __int_as_float((__float_as_int(x) + 0x7fffff) & 0x7f800000);
+}
+__device__ __forceinline__ float inverse_power(float x) { return __int_as_float(0x7f000000 - __float_as_int(x)); }
+
 struct Work {
   float* acc;   // [2 * grid][tile][hd]
   float* ml;    // [2 * grid][tile][2]
@@ -577,9 +583,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
         // 2^-60 at least of the largest unit that the sums have had, however often it falls: a page of zeros
         // has 2^-110, and the sums (2^15 * 448 a key) times all falls stay below 2^104 for 2^20 keys.
         least = fmaxf(least, v_unit * 0x1p-60f);
-        const float now = fmaxf(v_unit, least);
-        ratio = unit / now;
-        pscale = v_unit / now;
+        const float now = power_of_two(fmaxf(v_unit, least)), inv = inverse_power(now);
+        ratio = unit * inv;
+        pscale = v_unit * inv;
         unit = now;
       }
       uint32_t pf[NQ][2][2];
