@@ -190,6 +190,7 @@ struct Args {
   Kv8Attention a;
   Div rep, hkv;    // query heads of a kv head; kv heads
   int page_shift;
+  float down;      // 2^-15 / (tokens of a table's row, rounded up to a power of two)
 };
 
 __device__ __forceinline__ int new_rows(const Kv8Attention& a, int r, int& first) {
@@ -697,7 +698,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
-        const float sum = group_sum(l[n][z]);
+        // Weights (2^15 at most) and their sums are kept below 1 from here on, so that no sum of p v passes the
+        // largest |v|: a mean of values of 2^120 is finite where their sum is not.
+        const float sum = group_sum(l[n][z]) * args.down;
         const int y = 8 * n + 2 * t + z;
         if (g == 0) {
           sh_m[warp][y] = m[n][z];
@@ -707,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
 #pragma unroll
           for (int j = 0; j < MT; ++j)
             *reinterpret_cast<float2*>(so + y * HD + g * (HD / 8) + 2 * j) =
-                make_float2(o[j][n][z] * unit, o[j][n][z + 2] * unit);
+                make_float2(o[j][n][z] * args.down * unit, o[j][n][z + 2] * args.down * unit);
         }
       }
     __syncthreads();
@@ -923,8 +926,9 @@ long kv8_attention_work(const Kv8Attention& a, int hd) {
 int launch_kv8_attention(const Kv8Cache& c, const Kv8Attention& a, cudaStream_t st) {
   if (a.rows < 1) return 0;
   if (c.page % kChunk || (c.page & (c.page - 1)) || a.grid < 1) return kErrBadArgsHost;
-  Args args{c, a, make_div(a.H / c.hkv), make_div(c.hkv), 0};
+  Args args{c, a, make_div(a.H / c.hkv), make_div(c.hkv), 0, 0x1p-15f};
   while ((1 << args.page_shift) < c.page) ++args.page_shift;
+  for (long n = 1; n < (long)a.width * c.page; n *= 2) args.down *= 0.5f;
   if (a.cluster) {
     if (c.hd == 64 && a.tile == 8) return launch<64, 1, true>(args, st);
     if (c.hd == 64 && a.tile == 16) return launch<64, 2, true>(args, st);

@@ -128,3 +128,17 @@ def test_attention_of_small_values_behind_large_ones(hd, drop):
     assert float(want.abs().max()) < 4 * 2.0 ** (2 * drop)
     # the bound's 1e-30 stays below 2^-8 of the least of these values (2^-56)
     O.close(attend(q.to(BF16).cuda(), d), want, O.attention_bound(want, s))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("r,hkv,n", SPLITS)
+def test_attention_of_the_largest_values(hd, r, hkv, n):
+    """Values of 2^120 and more: a mean of them is finite, whatever their sum is."""
+    g = torch.Generator().manual_seed(6)
+    k = 0.3 * torch.randn(r, n, hkv, hd, generator=g)
+    v = (1 + 0.9 * torch.rand(r, n, hkv, hd, generator=g)) * 2.0**120
+    v[:, ::2, :, ::3] *= -1
+    d = appended([n] * r, k, v, 64)
+    q = torch.randn(r, hkv, hd, generator=g).to(BF16)
+    want, s = O.attention64(q, {x: y.cpu() for x, y in d.items()})
+    O.close(attend(q.cuda(), d), want, O.attention_bound(want, s))
