@@ -328,13 +328,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
     total = a.R * same;
     __syncthreads();
   } else {
-    // Steps (with CLUSTER segments) before each request, each thread's requests in a row. Ascending
-    // starts keep the sum below the host's bound; with any other nothing is computed.
+    // Steps (with CLUSTER segments) before each request, each thread's requests in a row. Starts that
+    // ascend within the rows keep the sum below the host's bound; with any other nothing is computed.
     const int per = (a.R + kThreads - 1) / kThreads;
     auto weight = [&](int r, int& bad) {
       int first;
       const int n = new_rows(a, r, first);
-      if (a.starts != nullptr) bad |= a.starts[r + 1] < first;
+      if (a.starts != nullptr) bad |= first < 0 || a.starts[r + 1] < first || a.starts[r + 1] > a.rows;
       return (n * rep + kRows - 1) / kRows * c.hkv * (CLUSTER ? 1 : steps_of(cap, a.lens[r]));
     };
     int mine = 0;
@@ -367,9 +367,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
   }
   if (!CLUSTER && blockIdx.x == 0)
     for (int r = tid; r <= a.R; r += kThreads) w.prefix[r] = prefix[r];
-  if (a.zero_tail) {  // rows of no request: before the first, behind the last, all if starts do not ascend
-    const int last = bad ? 0 : max(0, min(a.rows, a.starts[a.R]));
-    const int lead = bad ? 0 : max(0, min(last, a.starts[0]));
+  if (a.zero_tail) {  // rows of no request: before the first, behind the last, all if starts are refused
+    const int last = bad ? 0 : a.starts[a.R];
+    const int lead = bad ? 0 : a.starts[0];
     constexpr int kPieces = HD / 8;
     const long per = (long)a.H * kPieces, n = (a.rows - last + lead) * per;
     uint4* o = reinterpret_cast<uint4*>(a.out);
@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
   wait_for_previous();
   int r = row;
   const int total = w.prefix[a.R];
-  if (total == 0) return;  // nothing was computed: starts that do not ascend, or no request has a row
+  if (total == 0) return;  // nothing was computed: starts are refused, or no request has a row
   if (a.starts != nullptr) {
     // Rows of no request. Before the first, row - starts[r] is negative: every index below would lie
     // before its array.

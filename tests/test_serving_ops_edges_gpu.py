@@ -142,3 +142,22 @@ def test_attention_of_the_largest_values(hd, r, hkv, n):
     q = torch.randn(r, hkv, hd, generator=g).to(BF16)
     want, s = O.attention64(q, {x: y.cpu() for x, y in d.items()})
     O.close(attend(q.cuda(), d), want, O.attention_bound(want, s))
+
+
+@pytest.mark.parametrize("starts", [[0, 8, 20], [-2, 3, 8], [0, 4, 9], [-1, -1, 8], [9, 9, 9], [0, 3, 2**31 - 1],
+                                    [-(2**31), 0, 2**31 - 1], [0, -(2**31), 8]])
+@pytest.mark.parametrize("lens", [[40, 50], [3000, 5000]])
+def test_attention_starts_outside_the_rows(starts, lens):
+    """Refused on the device, like those that do not ascend: nothing is computed, and without ``out``
+    every row is zero."""
+    c = O.make_cache(lens, hkv=1, hd=64, page=32, seed=1)
+    q = torch.randn(8, 2, 64, generator=torch.Generator().manual_seed(1)).to(BF16)
+    d = cuda(c)
+    out = torch.full((8, 2, 64), 3.0, dtype=BF16, device="cuda")
+    attend(q.cuda(), d, starts=ints(starts), out=out)
+    assert bool((out == 3).all())
+    # what an earlier tensor held is not what comes out
+    junk = torch.full((8, 2, 64), 5.0, dtype=BF16, device="cuda")
+    del junk
+    assert not bool(attend(q.cuda(), d, starts=ints(starts)).any())
+    assert not bool(attend(q, c, starts=torch.tensor(starts, dtype=torch.int32)).any())
