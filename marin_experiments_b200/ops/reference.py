@@ -360,9 +360,10 @@ def block_tables_extend(tables, lens, new_lens, free_pages, free_count, page: in
 
 def block_tables_release(tables, lens, done, free_pages, free_count, page: int):
     """See ``api.block_tables_release``."""
-    n = [-(-a // page) if d else 0 for a, d in zip(lens.tolist(), done.tolist())]
+    gone = [a if d else 0 for a, d in zip(lens.tolist(), done.tolist())]
+    n = [max(0, -(-a // page)) for a in gone]
     count, status = int(free_count), 0
-    if not 0 <= count <= free_pages.numel() or min(n) < 0 or sum(n) > free_pages.numel() - count:
+    if not 0 <= count <= free_pages.numel() or min(gone) < 0 or sum(n) > free_pages.numel() - count:
         status |= TABLES_BAD_INPUT
     if max(n) > tables.shape[1]:
         status |= TABLES_TOO_LONG

@@ -161,3 +161,17 @@ def test_attention_starts_outside_the_rows(starts, lens):
     del junk
     assert not bool(attend(q.cuda(), d, starts=ints(starts)).any())
     assert not bool(attend(q, c, starts=torch.tensor(starts, dtype=torch.int32)).any())
+
+
+@pytest.mark.parametrize("lens,done,count", [([-3, 5], [True, False], 1), ([-64, 5], [True, False], 1),
+                                             ([3, -1], [True, True], 1), ([200, 5], [True, True], 1),
+                                             ([200, -5], [True, True], 3), ([3, 5], [True, True], 9),
+                                             ([3, 5], [True, True], -1), ([100, 100], [True, True], 3),
+                                             ([-3, 5], [False, True], 1), ([2**31 - 1] * 2, [True, True], 1)])
+def test_tables_release_refuses_like_the_cpu(lens, done, count):
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    host = [i32([[5, 4], [2, 7]]), i32(lens), torch.tensor(done), i32([9, 0, 0, 0, 0, 0]), i32([count])]
+    dev = [t.cuda() for t in host]
+    assert int(api.block_tables_release(*dev, 64)) == int(api.block_tables_release(*host, 64))
+    for a, b in zip(host, dev):
+        assert torch.equal(a, b.cpu())
