@@ -427,12 +427,12 @@ def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, tables, lens, starts=No
         a, b = st[r], st[r + 1]
         for i in range(a, b):
             m = max(0, n - (b - 1 - i))
-            pg = tables[r, : -(-m // page)].long()
-            if m > tables.shape[1] * page or bool(((pg < 0) | (pg >= pages)).any()):
-                o[i] = float("nan")
-                continue
             if m == 0:
                 o[i] = 0
+                continue
+            pg = tables[r, : -(-m // page)].long()
+            if n > tables.shape[1] * page or bool(((pg < 0) | (pg >= pages)).any()):
+                o[i] = float("nan")
                 continue
             kk, vv = ((c[pg].float() * s[pg].abs()[..., None, None]).transpose(1, 2).reshape(-1, hkv, hd)[:m]
                       for c, s in ((k_cache, k_scale), (v_cache, v_scale)))

@@ -27,3 +27,21 @@ def test_tables_release_refuses(lens, done, count, status):
     assert int(api.block_tables_release(*state, 64)) == status
     if status:
         assert all(torch.equal(a, b) for a, b in zip(state, before))
+
+
+def long_request(new):
+    """A request longer than its table (64 tokens in two pages of 32), beside an ordinary one."""
+    c = O.make_cache([64, 40], hkv=1, hd=64, page=32, seed=2)
+    c["tables"] = c["tables"][:, :2].contiguous()
+    c["lens"][0] = 65
+    q = torch.randn(new + 1, 2, 64, generator=torch.Generator().manual_seed(1)).to(BF16)
+    return c, q, ints([0, new, new + 1])
+
+
+@pytest.mark.parametrize("new", [1, 3, 64, 65, 67])
+def test_attention_of_a_request_longer_than_its_table(new):
+    """All of its rows that see a token are NaN, also those whose tokens the table holds."""
+    c, q, starts = long_request(new)
+    got = api.kv8_attention(q, c["k"], c["v"], c["ks"], c["vs"], c["tables"], c["lens"], starts=starts)
+    blind = max(0, new - 65)
+    assert not bool(got[:blind].any()) and bool(torch.isnan(got[blind:new]).all()) and bool(torch.isfinite(got[new]).all())

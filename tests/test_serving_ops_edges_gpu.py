@@ -175,3 +175,20 @@ def test_tables_release_refuses_like_the_cpu(lens, done, count):
     assert int(api.block_tables_release(*dev, 64)) == int(api.block_tables_release(*host, 64))
     for a, b in zip(host, dev):
         assert torch.equal(a, b.cpu())
+
+
+@pytest.mark.parametrize("more", [0, 300])  # requests: a cluster each, or shared among all CTAs
+@pytest.mark.parametrize("new", [1, 3, 64, 65, 67])
+def test_attention_of_a_request_longer_than_its_table(new, more):
+    """All of its rows that see a token are NaN, on the CPU too."""
+    lens = [64, 40] + [33] * more
+    c = O.make_cache(lens, hkv=2, hd=64, page=32, seed=2)
+    c["tables"] = c["tables"][:, :2].contiguous()
+    c["lens"][0] = 65
+    starts = [0, new] + [new + 1 + i for i in range(more + 1)]
+    q = torch.randn(new + 1 + more, 4, 64, generator=torch.Generator().manual_seed(1)).to(BF16)
+    want = attend(q, c, starts=torch.tensor(starts, dtype=torch.int32))
+    got = attend(q.cuda(), cuda(c), starts=ints(starts)).cpu()
+    blind = max(0, new - 65)
+    assert bool(torch.isnan(got[blind:new]).all()) and torch.equal(torch.isnan(got), torch.isnan(want))
+    assert not bool(got[:blind].any()) and not bool(want[:blind].any())
