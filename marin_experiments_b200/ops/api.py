@@ -296,7 +296,7 @@ def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, tables, lens, *, starts
     ``starts[r] .. starts[r + 1]`` of ``q`` are the last tokens of request r; without ``starts`` each
     request has one row. A row that sees no token is zero. A row that sees a page outside the cache is
     NaN, and so is every other row of a request that is longer than its table. Rows of no request (before ``starts[0]``, behind
-    ``starts[R]``) are left as they were in ``out``, and are zero without it. ``starts`` must ascend
+    ``starts[R]``) are left as they were in ``out`` (which overlaps no input), and are zero without it. ``starts`` must ascend
     within ``0 .. rows``; with others nothing is computed. The cache is one that ``kv8_append`` wrote:
     scales are powers of two, and a page of values with NaN codes has a negative one."""
     _serving_only("kv8_attention", q)

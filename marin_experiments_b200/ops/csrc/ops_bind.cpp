@@ -559,9 +559,15 @@ void same_device(const Tensor& a, std::initializer_list<const Tensor*> rest) {
 Tensor fresh(c10::IntArrayRef sizes, const Tensor& on, at::ScalarType type) {
   return at::detail::empty_cuda(sizes, type, on.device(), std::nullopt);
 }
+// a is contiguous; b is too, but for the stride of its first dimension.
 bool overlaps(const Tensor& a, const Tensor& b) {
-  const char *x = (const char*)a.data_ptr(), *y = (const char*)b.data_ptr();
-  return x < y + b.nbytes() && y < x + a.nbytes();
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const int64_t x = (int64_t)a.data_ptr(), y = (int64_t)b.data_ptr(), end = x + (int64_t)a.nbytes();
+  const int64_t n = b.dim() ? b.size(0) : 1, row = (int64_t)b.nbytes() / n;
+  const int64_t step = n > 1 ? b.stride(0) * (int64_t)b.element_size() : 0;
+  if (step == 0 || step == row) return x < y + row + (n - 1) * step && y < end;
+  const int64_t i = x < y + row ? 0 : (x - y - row) / step + 1;  // the first row of b that ends behind a's start
+  return i < n && y + i * step < end;
 }
 
 std::vector<Tensor> block_tables_extend(const Tensor& tables, const Tensor& lens, const Tensor& grow,
@@ -702,7 +708,8 @@ Tensor kv8_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const 
     aligned16(o, "out");
     same_device(kc, {&o});
     need(o.sizes() == q.sizes(), "out must have q's shape");
-    need(!overlaps(o, kc) && !overlaps(o, vc) && (T == 0 || !overlaps(o, q)), "out must not overlap an input");
+    for (auto* t : {&q, &kc, &vc, &ks, &vs, &tables, &lens}) need(!overlaps(o, *t), "out must not overlap an input");
+    need(!starts.has_value() || !overlaps(o, *starts), "out must not overlap an input");
   } else {
     o = fresh(q.sizes(), q, at::kBFloat16);
   }

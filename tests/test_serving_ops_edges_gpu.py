@@ -192,3 +192,27 @@ def test_attention_of_a_request_longer_than_its_table(new, more):
     blind = max(0, new - 65)
     assert bool(torch.isnan(got[blind:new]).all()) and torch.equal(torch.isnan(got), torch.isnan(want))
     assert not bool(got[:blind].any()) and not bool(want[:blind].any())
+
+
+def test_attention_out_inside_the_rows_of_q():
+    """q may be a slice of wider rows: an out that lies behind its first rows overlaps it all the same,
+    one that lies between two rows does not."""
+    c = cuda(O.make_cache([40, 50, 7], hkv=2, hd=64, page=32))
+    h, hd = 4, 64
+    buf = torch.randn(3 * 2 * h * hd + 64, device="cuda").to(BF16)
+    q = buf[: 3 * 2 * h * hd].view(3, 2 * h * hd)[:, : h * hd].view(3, h, hd)
+    want = attend(q, c)
+    for at in (0, 8, h * hd - 8, 3 * h * hd):  # the last: behind q.numel() elements from q's start
+        with pytest.raises(RuntimeError, match="overlap"):
+            attend(q, c, out=buf[at: at + 3 * h * hd].view(3, h, hd))
+    wide = torch.randn(3, 4 * h * hd, device="cuda").to(BF16)
+    wide[:, : h * hd] = q.reshape(3, -1)
+    out = wide.view(-1)[h * hd: 4 * h * hd].view(3, h, hd)
+    assert torch.equal(attend(wide[:, : h * hd].view(3, h, hd), c, out=out), want)
+    back = wide.view(-1)[h * hd - 8: 4 * h * hd - 8].view(3, h, hd)
+    with pytest.raises(RuntimeError, match="overlap"):
+        attend(wide[:, : h * hd].view(3, h, hd), c, out=back)
+    with pytest.raises(RuntimeError, match="overlap"):
+        attend(want, c, out=want)
+    with pytest.raises(RuntimeError, match="overlap"):
+        attend(q, c, out=c["k"].view(-1).view(BF16)[: 3 * h * hd].view(3, h, hd))
