@@ -272,7 +272,7 @@ def block_tables_release(tables, lens, done, free_pages, free_count, page_size: 
 def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, slots) -> None:
     """Write rows of keys and values (``[rows, kv_heads, head_dim]`` bf16, head_dim 64 or 128) to
     their slots of a cache of e4m3 codes ``[pages, kv_heads, page, head_dim]`` (page 32, 64 or 128)
-    with fp32 scales ``[pages, kv_heads]``, in place.
+    with fp32 scales ``[pages, kv_heads]``, in place. Keys and values have caches and scales of their own.
 
     Scales are powers of two. A row at offset 0 starts its page anew; rows further on keep the page's
     scale or raise it, and raising it rescales the codes before them. Values that are not finite are

@@ -672,6 +672,7 @@ void kv8_append(const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor
   const long kt = rows_of(k, c.hkv, c.hd, "k"), vt = rows_of(v, c.hkv, c.hd, "v");
   cuda_i32(slots, "slots");
   same_device(kc, {&k, &v, &slots});
+  need(!overlaps(kc, vc) && !overlaps(ks, vs), "the caches of keys and values must not overlap");
   need(k.size(0) == v.size(0) && slots.dim() == 1 && slots.size(0) == k.size(0), "one slot for each row of k and v");
   need(k.size(0) <= 1LL << 30, "more than 2^30 rows");
   c10::cuda::CUDAGuard g(kc.device());

@@ -216,3 +216,12 @@ def test_attention_out_inside_the_rows_of_q():
         attend(want, c, out=want)
     with pytest.raises(RuntimeError, match="overlap"):
         attend(q, c, out=c["k"].view(-1).view(BF16)[: 3 * h * hd].view(3, h, hd))
+
+
+def test_append_to_one_cache_twice():
+    """Keys and values need caches of their own."""
+    c = cuda(O.make_cache([40], hkv=1, hd=64, page=32))
+    k = torch.ones(1, 1, 64, device="cuda", dtype=BF16)
+    for a, b, s, t in (("k", "k", "ks", "vs"), ("k", "v", "ks", "ks")):
+        with pytest.raises(RuntimeError, match="overlap"):
+            api.kv8_append(k, k, c[a], c[b], c[s], c[t], ints([0]))
