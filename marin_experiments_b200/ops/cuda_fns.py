@@ -641,4 +641,5 @@ def linear_w4_dense(x, codes, scales, residual, glu):
     if residual is None:
         return G.linear(x, w)
     out = torch.empty(t, n, dtype=BF16, device=x.device)
-    return G.linear(x, w, out=out, epi="resid", r=_c(residual))
+    # the GEMM has no tile of 64 columns that adds a residual
+    return G.linear(x, w, out=out, epi="resid", r=_c(residual), bn=128 if n < 128 else None)

@@ -225,3 +225,31 @@ def test_append_to_one_cache_twice():
     for a, b, s, t in (("k", "k", "ks", "vs"), ("k", "v", "ks", "ks")):
         with pytest.raises(RuntimeError, match="overlap"):
             api.kv8_append(k, k, c[a], c[b], c[s], c[t], ints([0]))
+
+
+def exact_w4(n, k, group, t, seed=0):
+    """Small whole numbers times powers of two: every sum of fewer than 2^24 / (4 * 8 * 4) values of K is
+    exact in fp32, in any order, so a result is the fp64 one rounded once."""
+    from marin_experiments_b200.ops.quant import pack_w4
+
+    assert 4 * 8 * 4 * k < 2**24
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randint(-8, 8, (n, k), generator=g)
+    scales = torch.exp2(torch.randint(0, 3, (n, k // group), generator=g).float()).to(BF16)
+    x = torch.randint(-4, 5, (t, k), generator=g).to(BF16)
+    w = (codes.double().view(n, -1, group) * scales.double()[..., None]).view(n, k)
+    res = (torch.randint(-200, 201, (t, n), generator=g) / 2).to(BF16)
+    return x, pack_w4(codes), scales, res, x.double() @ w.t()
+
+
+@pytest.mark.parametrize("t", [65, 130])
+@pytest.mark.parametrize("n", [32, 64, 96, 128, 256])
+def test_linear_w4_many_rows_round_once(t, n):
+    """The residual is added before the one rounding, at every width."""
+    x, codes, scales, res, y = exact_w4(n, 512, 64, t)
+    got = api.linear_w4(x.cuda(), codes.cuda(), scales.cuda(), residual=res.cuda())
+    assert torch.equal(got.cpu(), (y + res.double()).to(BF16)) and got.is_contiguous()
+    wide = torch.zeros(t, n + 5, dtype=BF16, device="cuda")
+    wide[:, 5:] = res.cuda()
+    assert torch.equal(api.linear_w4(x.cuda(), codes.cuda(), scales.cuda(), residual=wide[:, 5:]), got)
+    assert torch.equal(api.linear_w4(x.cuda(), codes.cuda(), scales.cuda()).cpu(), y.to(BF16))
