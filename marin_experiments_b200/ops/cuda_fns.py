@@ -636,10 +636,12 @@ def linear_w4_dense(x, codes, scales, residual, glu):
     pad = -n % 32  # the GEMM stores 32 columns at a time
     if pad:
         w = torch.cat([w, w.new_zeros(pad, k)])
-        out = G.linear(x, w)[:, :n]
-        return (out if residual is None else out + residual).contiguous()
+        if residual is not None:  # padded too: the GEMM adds it before its one rounding
+            residual = torch.cat([residual, residual.new_zeros(t, pad)], 1)
     if residual is None:
-        return G.linear(x, w)
-    out = torch.empty(t, n, dtype=BF16, device=x.device)
-    # the GEMM has no tile of 64 columns that adds a residual
-    return G.linear(x, w, out=out, epi="resid", r=_c(residual), bn=128 if n < 128 else None)
+        out = G.linear(x, w)
+    else:
+        out = torch.empty(t, n + pad, dtype=BF16, device=x.device)
+        # the GEMM has no tile of 64 columns that adds a residual
+        G.linear(x, w, out=out, epi="resid", r=_c(residual), bn=128 if n + pad < 128 else None)
+    return out[:, :n].contiguous() if pad else out

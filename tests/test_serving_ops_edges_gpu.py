@@ -243,9 +243,9 @@ def exact_w4(n, k, group, t, seed=0):
 
 
 @pytest.mark.parametrize("t", [65, 130])
-@pytest.mark.parametrize("n", [32, 64, 96, 128, 256])
+@pytest.mark.parametrize("n", [1, 32, 33, 64, 96, 100, 128, 256, 1000])
 def test_linear_w4_many_rows_round_once(t, n):
-    """The residual is added before the one rounding, at every width."""
+    """The residual is added before the one rounding, at widths that the dense GEMM does not store too."""
     x, codes, scales, res, y = exact_w4(n, 512, 64, t)
     got = api.linear_w4(x.cuda(), codes.cuda(), scales.cuda(), residual=res.cuda())
     assert torch.equal(got.cpu(), (y + res.double()).to(BF16)) and got.is_contiguous()
