@@ -253,3 +253,15 @@ def test_linear_w4_many_rows_round_once(t, n):
     wide[:, 5:] = res.cuda()
     assert torch.equal(api.linear_w4(x.cuda(), codes.cuda(), scales.cuda(), residual=wide[:, 5:]), got)
     assert torch.equal(api.linear_w4(x.cuda(), codes.cuda(), scales.cuda()).cpu(), y.to(BF16))
+
+
+@pytest.mark.parametrize("n,k,t,group", [(20, 98304, 3, 32), (20, 98304, 3, 128), (5, 98304, 20, 64), (300, 98304, 40, 32),
+                                         (70, 12288, 33, 32), (33, 14336, 64, 128), (40, 8192, 1, 64), (4096, 4096, 8, 128),
+                                         (5000, 1152, 16, 32), (129, 16384, 31, 128)])
+def test_linear_w4_is_exact_on_whole_numbers(n, k, t, group):
+    """Bit for bit, so that a slice of K left out or taken twice shows at any K (a bound on the rounding
+    errors of 98304 additions is as large as a result there)."""
+    x, codes, scales, res, y = exact_w4(n, k, group, t)
+    c, s = codes.cuda(), scales.cuda()
+    assert torch.equal(api.linear_w4(x.cuda(), c, s).cpu(), y.to(BF16))
+    assert torch.equal(api.linear_w4(x.cuda(), c, s, residual=res.cuda()).cpu(), (y + res.double()).to(BF16))
