@@ -265,3 +265,53 @@ def test_linear_w4_is_exact_on_whole_numbers(n, k, t, group):
     c, s = codes.cuda(), scales.cuda()
     assert torch.equal(api.linear_w4(x.cuda(), c, s).cpu(), y.to(BF16))
     assert torch.equal(api.linear_w4(x.cuda(), c, s, residual=res.cuda()).cpu(), (y + res.double()).to(BF16))
+
+
+@pytest.mark.parametrize("h,hkv,hd,page,lens,new", [
+    # tiles of 16 rows, segments shared among all CTAs
+    (96, 8, 128, 64, [300] * 20 + [1, 0, 129] * 7, None), (96, 8, 64, 64, [300] * 30 + [1, 0, 129] * 10, None),
+    (16, 1, 64, 32, [300] * 440 + [5000], None),
+    (8, 2, 128, 64, [6000, 2500], [3, 4]), (8, 2, 64, 32, [6000, 2500], [3, 4]),
+    (4, 2, 128, 64, [9000], [8]), (4, 2, 64, 64, [9000], [8]),
+    # in clusters of four and of one
+    (12, 4, 128, 128, [4000, 130, 33] * 3, [5, 1, 4] * 3), (20, 2, 128, 64, [900] * 90, None),
+    # tiles of 32
+    (32, 1, 64, 64, [3000, 700], [2, 1])])
+def test_attention_tiles_of_many_rows(h, hkv, hd, page, lens, new):
+    """9 and more query rows a kv head, over contexts that several CTAs share, with leading and trailing
+    rows of no request where there are several a request."""
+    c = O.make_cache(lens, hkv=hkv, hd=hd, page=page, seed=21)
+    d = cuda(c)
+    starts, rows = None, len(lens)
+    if new is not None:
+        starts = [5]
+        for n in new:
+            starts.append(starts[-1] + n)
+        rows = starts[-1] + 3
+    q = torch.randn(rows, h, hd, generator=torch.Generator().manual_seed(2)).to(BF16)
+    want, size = O.attention64(q, c, starts)
+    st = None if starts is None else ints(starts)
+    got = attend(q.cuda(), d, starts=st)
+    O.close(got, want, O.attention_bound(want, size))
+    assert torch.equal(got, attend(q.cuda(), d, starts=st))  # bit for bit
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("h,hkv,r,new", [(12, 1, 2, 1), (4, 2, 1, 7), (96, 8, 38, 1), (3, 1, 1, 11)])
+def test_attention_tiles_of_many_rows_with_nan_and_zeros(h, hkv, hd, r, new):
+    """Tokens whose values are zero for 256 tokens at a time, and values that are not finite: one that all
+    rows see, one among the newest tokens that the earlier rows do not."""
+    g = torch.Generator().manual_seed(8)
+    n = 2500 if r < 10 else 700
+    k = 0.3 * torch.randn(r, n, hkv, hd, generator=g)
+    v = 1 + torch.randn(r, n, hkv, hd, generator=g)
+    v[:, torch.arange(n) % 384 >= 128] = 0
+    v[0, 130, 0, 5], v[r - 1, n - 3, hkv - 1, hd - 1] = float("inf"), float("nan")
+    d = appended([n] * r, k, v, 64)
+    starts = [i * new for i in range(r + 1)]
+    q = torch.randn(r * new, h, hd, generator=g).to(BF16)
+    want, size = O.attention64(q, {x: y.cpu() for x, y in d.items()}, starts)
+    rep = h // hkv
+    seen = max(0, min(new, 3))  # rows that see the token n - 3
+    assert int(torch.isnan(want).sum()) == rep * (new + seen)
+    O.close(attend(q.cuda(), d, starts=ints(starts)), want, O.attention_bound(want, size))
