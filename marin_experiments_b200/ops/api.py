@@ -278,8 +278,9 @@ def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, slots) -> None:
     scale or raise it, and raising it rescales the codes before them. Values that are not finite are
     stored as NaN, and a page that holds such a value (not a key) gets a negative ``v_scale``. Rows
     with a slot outside the cache (the padding's -1) are skipped. The rows of one page must be
-    consecutive rows with ascending slots, as a ``BlockPlan`` gives them, and a page must belong to
-    one request: two runs of rows in one page would race for its scale."""
+    consecutive rows, each with the slot that follows the last one's, as a ``BlockPlan`` gives them, and
+    a page must belong to one request: two runs of rows in one page (a gap between their slots makes
+    two) would race for its scale."""
     _serving_only("kv8_append", k, v)
     if k.is_cuda:
         _cuda().ext().kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, slots)
