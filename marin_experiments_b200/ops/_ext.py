@@ -46,7 +46,10 @@ def err_flag(device: torch.device) -> torch.Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     t = _ERR.get(idx)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        dev = torch.device("cuda", idx)
+        # A first call may be made in inference mode, whose tensors cannot be cleared outside it.
+        with torch.inference_mode(False), torch.cuda.device(dev):
+            t = torch.zeros(1, dtype=torch.int32, device=dev)
         _ERR[idx] = t
     return t
 

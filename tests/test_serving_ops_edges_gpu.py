@@ -1,6 +1,10 @@
 """Calls of the quantised serving operators at the edges of what their documentation allows, against
 fp64 definitions."""
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -10,6 +14,7 @@ import serving_ops_oracle as O
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def ints(v):
@@ -315,3 +320,34 @@ def test_attention_tiles_of_many_rows_with_nan_and_zeros(h, hkv, hd, r, new):
     seen = max(0, min(new, 3))  # rows that see the token n - 3
     assert int(torch.isnan(want).sum()) == rep * (new + seen)
     O.close(attend(q.cuda(), d, starts=ints(starts)), want, O.attention_bound(want, size))
+
+
+FIRST_CALL = """
+import torch
+from marin_experiments_b200.ops import api, _ext
+codes, scales = (t.cuda() for t in api.quantize_w4(torch.randn(256, 256), 64))
+x = torch.randn(40, 256, device="cuda").to(torch.bfloat16)
+torch.cuda.synchronize()
+{how}
+flag = _ext.err_flag(x.device)
+flag.fill_(61)  # as a wait that gave up in a kernel before
+{again}
+try:
+    _ext.check_kernel_errors()
+    raise SystemExit("the record is lost")
+except _ext.KernelTimeoutError:
+    pass
+_ext.check_kernel_errors()  # cleared
+want = api.linear_w4(x[:20].contiguous(), codes, scales)
+assert (out[:20].float() - want.float()).abs().max() < 0.05 * want.float().abs().max()
+"""
+
+
+@pytest.mark.parametrize("how,again", [
+    ("with torch.inference_mode():\n    out = api.linear_w4(x, codes, scales)", "")])
+def test_the_error_flag_of_a_first_call_that_is_captured_or_in_inference_mode(how, again):
+    """The flag of timed-out waits is no graph's memory (a replay would clear it) and no inference
+    tensor (which the check could not clear)."""
+    code = FIRST_CALL.format(how=how, again=again)
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0, r.stderr[-2000:]
