@@ -47,9 +47,10 @@ def err_flag(device: torch.device) -> torch.Tensor:
     t = _ERR.get(idx)
     if t is None:
         dev = torch.device("cuda", idx)
-        # A first call may be made in inference mode, whose tensors cannot be cleared outside it.
+        # A first call may be made in inference mode, whose tensors cannot be cleared outside it, or captured:
+        # zeros of the captured stream would be the graph's, which would clear the flag at each replay.
         with torch.inference_mode(False), torch.cuda.device(dev):
-            t = torch.zeros(1, dtype=torch.int32, device=dev)
+            t = ext().kept_flag() if torch.cuda.is_current_stream_capturing() else torch.zeros(1, dtype=torch.int32, device=dev)
         _ERR[idx] = t
     return t
 

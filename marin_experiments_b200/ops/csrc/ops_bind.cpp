@@ -35,6 +35,26 @@ T* ptr(const OptT& t) {
 // locale facets are not this library's own) instead of raising.
 void ok(int code, const char* what) { TORCH_CHECK(code == 0, what, " failed (", std::to_string(code), ")"); }
 
+// A zeroed int32 of the current device that no graph owns, also while its stream is being captured: the capture
+// lets this thread use other streams meanwhile. It lives as long as the process.
+Tensor kept_flag() {
+  struct Relaxed {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    Relaxed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~Relaxed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  } relaxed;
+  void* p = nullptr;
+  cudaStream_t side = nullptr;
+  bool fine = cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking) == cudaSuccess;
+  fine = fine && cudaMalloc(&p, sizeof(int)) == cudaSuccess && cudaMemsetAsync(p, 0, sizeof(int), side) == cudaSuccess &&
+         cudaStreamSynchronize(side) == cudaSuccess;
+  if (side != nullptr) cudaStreamDestroy(side);
+  need(fine, "no memory for the error flag");
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return torch::from_blob(p, {1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, dev));
+}
+
 // ------------------------------------------------------------------------------------ rows
 void rmsnorm_fwd(const Tensor& x, const Tensor& w, const Tensor& y, const Tensor& rstd, double eps) {
   cuda_bf16(x, "x"); cuda_f32(w, "w"); cuda_bf16(y, "y"); cuda_f32(rstd, "rstd");
@@ -869,6 +889,7 @@ void register_ops(pybind11::module& m) {
   m.def("kv8_attention", &kv8_attention);
   m.def("linear_w4", &linear_w4);
   m.def("dequant_w4", &dequant_w4);
+  m.def("kept_flag", &kept_flag);
   m.def("ipc_alloc", &ipc_alloc);
   m.def("ipc_open", &ipc_open);
   m.def("ipc_close", [](int64_t p) { return mxk::ipc_close(reinterpret_cast<void*>(p)); });

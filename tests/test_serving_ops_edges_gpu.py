@@ -344,6 +344,8 @@ assert (out[:20].float() - want.float()).abs().max() < 0.05 * want.float().abs()
 
 
 @pytest.mark.parametrize("how,again", [
+    ("g = torch.cuda.CUDAGraph()\nwith torch.cuda.graph(g):\n    out = api.linear_w4(x, codes, scales)\n"
+     "_ext.check_kernel_errors()", "g.replay()"),
     ("with torch.inference_mode():\n    out = api.linear_w4(x, codes, scales)", "")])
 def test_the_error_flag_of_a_first_call_that_is_captured_or_in_inference_mode(how, again):
     """The flag of timed-out waits is no graph's memory (a replay would clear it) and no inference
