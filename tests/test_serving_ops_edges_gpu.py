@@ -353,3 +353,54 @@ def test_the_error_flag_of_a_first_call_that_is_captured_or_in_inference_mode(ho
     code = FIRST_CALL.format(how=how, again=again)
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=240)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("starts", [False, True])
+def test_the_most_requests_of_a_call(starts):
+    """4096 requests, among them empty ones and one that is long."""
+    r = 4096
+    lens = [(7 * i) % 70 for i in range(r)]
+    lens[1234] = 4000
+    c = O.make_cache(lens, hkv=1, hd=64, page=32, seed=1)
+    new = [i % 3 for i in range(r)] if starts else [1] * r
+    first = [0]
+    for n in new:
+        first.append(first[-1] + n)
+    q = torch.randn(first[-1], 2, 64, generator=torch.Generator().manual_seed(2)).to(BF16)
+    want, size = O.attention64(q, c, first)
+    got = attend(q.cuda(), cuda(c), starts=ints(first) if starts else None)
+    O.close(got, want, O.attention_bound(want, size))
+
+
+def test_a_step_without_new_tokens():
+    """Nothing is placed, and nothing but the lengths comes out."""
+    tables, lens = ints([[5, 4], [6, -1]]), ints([70, 3])
+    p = api.block_tables_extend(tables, lens, ints([0, 0]), ints([9, 0]), ints([1]), 64, 0)
+    assert int(p.status) == 0 and p.lens.tolist() == [70, 3] and p.starts.tolist() == [0, 0, 0]
+    assert int(p.free_count) == 1 and p.slots.numel() == 0 and tables.tolist() == [[5, 4], [6, -1]]
+
+
+def test_attention_in_two_graphs_beside_an_eager_call():
+    """Graphs of shared segments (with workspaces) and of clusters replay beside one another, over lengths
+    that change between the replays."""
+    c = [cuda(O.make_cache([n, 40, 700], hkv=2, hd=128, page=64, seed=s)) for n, s in ((5000, 1), (5000, 2), (900, 3))]
+    q = [torch.randn(3, 8, 128, generator=torch.Generator().manual_seed(s)).to(BF16).cuda() for s in (1, 2, 3)]
+    graphs, outs = [], []
+    for i in range(3):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(attend(q[i], c[i]))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for step in range(8):
+        for x in c:
+            x["lens"].sub_(step)
+        want = [attend(q[i], c[i]) for i in range(3)]
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        with torch.cuda.stream(streams[3]):
+            eager = attend(q[0], c[0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip([*outs, eager], [*want, want[0]])), step
