@@ -299,7 +299,10 @@ def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, tables, lens, *, starts
     NaN, and so is every other row of a request that is longer than its table. Rows of no request (before ``starts[0]``, behind
     ``starts[R]``) are left as they were in ``out`` (which overlaps no input), and are zero without it. ``starts`` must ascend
     within ``0 .. rows``; with others nothing is computed. The cache is one that ``kv8_append`` wrote:
-    scales are powers of two, and a page of values with NaN codes has a negative one."""
+    scales are powers of two, and a page of values with NaN codes has a negative one.
+
+    Scores, softmax sums and outputs are summed in fp32; the weights meet the values rounded to f16
+    (2^-12 of a weight), well inside the result's own rounding to bf16."""
     _serving_only("kv8_attention", q)
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
@@ -313,8 +316,10 @@ def linear_w4(x, codes, scales, *, residual=None, glu: bool = False) -> torch.Te
 
     ``glu``: the weight holds block-interleaved gate and up rows (``ops.layout``) and the result is
     ``silu(gate) * up`` ``[T, N / 2]``. Up to 64 rows the weights stay in 4 bits on their way to the
-    tensor cores; more rows run the dense GEMM on weights written out in bf16 (each rounded once
-    more, and a temporary of ``2 N K`` bytes)."""
+    tensor cores (rows of ``x`` start at multiples of 16 bytes); more rows run the dense GEMM on
+    weights written out in bf16 (each rounded once more, and a temporary of ``2 N K`` bytes, which
+    takes longer than the GEMM on bf16 weights: it is for prompts of a model that has only these).
+    The residual is added in fp32, before the one rounding of the result."""
     _serving_only("linear_w4", x, residual)
     if not x.is_cuda:
         return R.linear_w4(x, codes, scales, residual, glu)

@@ -1,4 +1,5 @@
-// Paged KV cache in 8 bits: append of new keys and values, and attention over the cache.
+// Paged KV cache in 8 bits: its format, and the append of new keys and values (kv8_attention.cu has the
+// attention over it).
 //
 // A page holds `page` tokens of one kv head as e4m3 codes, [pages][hkv][page][hd], with one fp32
 // scale for each page and head, keys and values apart. A value is code * scale. Scales are powers of

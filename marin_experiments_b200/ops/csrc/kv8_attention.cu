@@ -55,7 +55,8 @@ constexpr int kManySteps = 16;
 // Most steps that a CTA of a cluster takes. Where clusters leave more than half of the GPU's places free,
 // sharing the steps among all places is worth the join's launch from three steps on (us, in clusters and
 // shared; one request of 2000 tokens, 8 kv heads: 8.35, 7.7; of 4000: 9.5, 8.3; two of 4000: 11.7, 9.7;
-// 1000 tokens, two steps: 6.8, 7.1). Where they fill it, not (16 requests of 500 to 2000 tokens: 15.5,
+// 1000 tokens, two steps: 6.5, 8.1; the rule sees the table's width and not the lengths, so a table wide enough
+// for 4096 tokens costs one of 1000 this). Where they fill it, not (16 requests of 500 to 2000 tokens: 15.5,
 // 17.5; 24 of 7 to 6001, 2 kv heads: 11.1, 12.3).
 constexpr int kClusterSteps = 16, kFewClusterSteps = 2;
 

@@ -12,12 +12,12 @@
 // 22), two issuing warps, stages of 256 values and a fifth stage were no faster. One thread found by
 // elect.sync with descriptors built once issues 20 % faster than lane 0 with descriptors built each time.
 //
-// The kernel for fewer rows (mma.sync) against this one, B200, device time in us:
+// The kernel for fewer rows (mma.sync) against this one, B200, device time in us (24576 with SwiGLU):
 //   rows, N x K, group      mma.sync  this      rows, N x K, group      mma.sync  this
-//   32, 4096 x 4096, 128        11.9  10.5      33, 4096 x 12288, 32        30.0  21.1
-//   32, 24576 x 4096, 128       34.2    44      64, 4096 x 12288, 128       36.8  22.5
-//   32, 4096 x 12288, 32        21.2    21      64, 24576 x 4096, 64        76.6  53.1
-// so up to 32 rows, where mma.sync needs four products for 128 weights, stay there.
+//   32, 4096 x 4096, 128        11.3  10.5      33, 4096 x 12288, 32        30.0  20.9
+//   32, 24576 x 4096, 128       33.7    44      64, 4096 x 12288, 128       36.8  22.4
+//   32, 4096 x 12288, 32        20.3    21      64, 24576 x 4096, 64        76.6  50.9
+// so up to 32 rows stay there: what this one gives at small N (8 %) is less than what it costs at large (30 %).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -42,7 +42,7 @@ constexpr int kRowsW = 128;              // rows of W of a CTA: M of the MMA
 constexpr int kStages = 4;
 constexpr int kCodeWarps = 8, kSumWarps = 4;
 constexpr int kCodes0 = 2, kSums0 = kCodes0 + kCodeWarps;
-constexpr int kAhead = 4;                // stages whose words are loaded ahead
+constexpr int kAhead = 4;                // stages whose words a thread loads ahead
 constexpr int kThreads = 32 * (kSums0 + kSumWarps);
 constexpr int kABytes = kRowsW * 256;    // two tiles of 64 values of K
 constexpr int kErrX = 61, kErrCodes = 62, kErrMma = 63, kErrSums = 64;
@@ -188,7 +188,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t* p[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) p[i] = a.codes + (long)min(row0 + r + 64 * i, a.N - 1) * (a.K / 8) + (long)b0 * 16 + 4 * t;
-    constexpr int kAhead = 4;
     uint4 w[kAhead][2];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)

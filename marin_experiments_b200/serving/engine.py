@@ -285,7 +285,8 @@ class Engine:
 
     @torch.no_grad()
     def refresh_weights(self) -> None:
-        """Copy the model's current weights into the engine's own (bf16) copies, in place: the
+        """Copy the model's current weights into the engine's own copies (rounded to 4 bits anew with
+        ``weights="int4"``), in place: the
         buffers, the KV caches and any captured decode graphs stay valid, so an RL learner can
         sample from its latest policy every step without rebuilding the engine. The CPU path reads
         the model directly and has nothing to copy."""
