@@ -10,7 +10,7 @@
 //
 // Exactness: e4m3 codes convert to f16 without rounding. A query row is multiplied by a power of two
 // that brings its largest value to 2^13, so its bf16 values are exact in f16 too (what is 2^-37 of
-// the row's largest rounds). Scores and sums are fp32. The weights p = 2^(s - max + 15) round to f16,
+// the row's largest rounds). Scores and sums are fp32. The weights 2^15 p, p = 2^(s - max), round to f16,
 // 2^-12 of a weight at most (below 2^-29 of the largest weight: absolutely). Output sums are held in
 // units of the current page's scale; a page of another scale rescales them by a power of two. The unit stays
 // above 2^-60 of the largest that a warp has met in the segment, so the weights of pages below 2^-89 of that lose
@@ -191,7 +191,7 @@ struct Args {
   Kv8Attention a;
   Div rep, hkv;    // query heads of a kv head; kv heads
   int page_shift;
-  float down;      // 2^-15 / (tokens of a table's row, rounded up to a power of two)
+  float down;      // 1 / (tokens of a table's row, rounded up to a power of two)
 };
 
 __device__ __forceinline__ int new_rows(const Kv8Attention& a, int r, int& first) {
@@ -590,6 +590,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
         pscale = v_unit * inv;
         unit = now;
       }
+      // Weights are at most 1 and meet the values as f16 times 2^15. The 15 is no part of the exponent: it would
+      // round away, or up to 32, beside scores of 2^24 and more.
+      pscale *= 0x1p15f;
       uint32_t pf[NQ][2][2];
       bool moved = false;
       float factor[NQ][2];
@@ -611,13 +614,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
 #pragma unroll
         for (int z = 0; z < 2; ++z)
           top[z] = fmaxf(fmaxf(s[0][n][z], s[0][n][z + 2]), fmaxf(s[1][n][z], s[1][n][z + 2]));
-        float sub[2];
+        float ref[2];
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
           const float mn = fmaxf(m[n][z], group_max(top[z]));
-          const float ref = mn == -INFINITY ? 0.f : mn;
-          const float alpha = ex2(m[n][z] - ref);
-          sub[z] = ref - 15.f;
+          ref[z] = mn == -INFINITY ? 0.f : mn;
+          const float alpha = ex2(m[n][z] - ref[z]);
           m[n][z] = mn;
           l[n][z] *= alpha;
           factor[n][z] = alpha * ratio;
@@ -627,13 +629,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
         for (int h = 0; h < 2; ++h) {
           float p[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) p[x] = ex2(s[h][n][x] - sub[x & 1]);
+          for (int x = 0; x < 4; ++x) p[x] = ex2(s[h][n][x] - ref[x & 1]);
           l[n][0] += p[0] + p[2];
           l[n][1] += p[1] + p[3];
-          if (pscale != 1.f) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) p[x] *= pscale;
-          }
+          for (int x = 0; x < 4; ++x) p[x] *= pscale;
           pf[n][h][0] = transpose8(pack_f16(p[0], p[1]));
           pf[n][h][1] = transpose8(pack_f16(p[2], p[3]));
         }
@@ -695,12 +695,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
     // join the warps: through shared memory, which the ring no longer needs
     __syncthreads();
     float* so = reinterpret_cast<float*>(smem) + warp * kRows * HD;
+    const float o_down = args.down * 0x1p-15f;
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
-        // Weights (2^15 at most) and their sums are kept below 1 from here on, so that no sum of p v passes the
-        // largest |v|: a mean of values of 2^120 is finite where their sum is not.
+        // The outputs' 2^15 goes, and the sum of a request's weights is kept below 1 from here on, so that no sum of
+        // p v passes the largest |v|: a mean of values of 2^120 is finite where their sum is not.
         const float sum = group_sum(l[n][z]) * args.down;
         const int y = 8 * n + 2 * t + z;
         if (g == 0) {
@@ -711,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, 8 * NQ, CLUSTER)) at
 #pragma unroll
           for (int j = 0; j < MT; ++j)
             *reinterpret_cast<float2*>(so + y * HD + g * (HD / 8) + 2 * j) =
-                make_float2(o[j][n][z] * args.down * unit, o[j][n][z + 2] * args.down * unit);
+                make_float2(o[j][n][z] * o_down * unit, o[j][n][z + 2] * o_down * unit);
         }
       }
     __syncthreads();
@@ -927,7 +928,7 @@ long kv8_attention_work(const Kv8Attention& a, int hd) {
 int launch_kv8_attention(const Kv8Cache& c, const Kv8Attention& a, cudaStream_t st) {
   if (a.rows < 1) return 0;
   if (c.page % kChunk || (c.page & (c.page - 1)) || a.grid < 1) return kErrBadArgsHost;
-  Args args{c, a, make_div(a.H / c.hkv), make_div(c.hkv), 0, 0x1p-15f};
+  Args args{c, a, make_div(a.H / c.hkv), make_div(c.hkv), 0, 1.f};
   while ((1 << args.page_shift) < c.page) ++args.page_shift;
   for (long n = 1; n < (long)a.width * c.page; n *= 2) args.down *= 0.5f;
   if (a.cluster) {

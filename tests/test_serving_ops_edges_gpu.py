@@ -404,3 +404,24 @@ def test_attention_in_two_graphs_beside_an_eager_call():
             eager = attend(q[0], c[0])
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip([*outs, eager], [*want, want[0]])), step
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("r,hkv,n", SPLITS)
+@pytest.mark.parametrize("size", [2.0**17, 2.0**22, 2.0**26, 2.0**31])
+def test_attention_of_very_large_scores(hd, r, hkv, n, size):
+    """Scores far beyond 2^24, whole numbers of which fp32 holds only every other and fewer: the weight is
+    on the keys of the largest score alone, eight of them with the same."""
+    g = torch.Generator().manual_seed(9)
+    k = torch.zeros(r, n, hkv, hd)
+    k[..., 0] = size / 2 * torch.rand(r, n, hkv, generator=g)
+    best = torch.rand(r, hkv, n, generator=g).topk(8, -1).indices
+    for i in range(r):
+        for j in range(hkv):
+            k[i, best[i, j], j, 0] = size
+    v = torch.randn(r, n, hkv, hd, generator=g)
+    d = appended([n] * r, k, v, 64)
+    q = torch.zeros(r, hkv, hd).to(BF16)
+    q[..., 0] = 1
+    want, s = O.attention64(q, {x: y.cpu() for x, y in d.items()}, scale=1.0)
+    O.close(attend(q.cuda(), d, scale=1.0), want, O.attention_bound(want, s))
