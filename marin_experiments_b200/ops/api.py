@@ -319,7 +319,8 @@ def linear_w4(x, codes, scales, *, residual=None, glu: bool = False) -> torch.Te
     tensor cores (rows of ``x`` start at multiples of 16 bytes); more rows run the dense GEMM on
     weights written out in bf16 (each rounded once more, and a temporary of ``2 N K`` bytes, which
     takes longer than the GEMM on bf16 weights: it is for prompts of a model that has only these).
-    The residual is added in fp32, before the one rounding of the result."""
+    The residual is added in fp32, before the one rounding of the result; with ``glu`` above 64 rows gate
+    and up are rounded to bf16 before the activation, as in ``dense_mlp``."""
     _serving_only("linear_w4", x, residual)
     if not x.is_cuda:
         return R.linear_w4(x, codes, scales, residual, glu)
