@@ -79,7 +79,7 @@ def appended(lens, k, v, page):
 
 # (requests, kv heads, tokens): long requests shared among all CTAs, a step of 128 keys each and many steps
 # each; clusters of 8 whose CTAs take three steps each; clusters of one CTA.
-SPLITS = [(2, 2, 5000), (40, 8, 3000), (4, 8, 3072), (37, 8, 1100)]
+SPLITS = [(2, 2, 5000), (40, 8, 3000), (4, 8, 3008), (37, 8, 1100)]
 
 
 @pytest.mark.parametrize("hd", [64, 128])
